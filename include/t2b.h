@@ -410,6 +410,106 @@ T2B_API int t2b_argmax_rows(const void* logits, int dtype, int M, int V, int ld,
                     size_t workspace_bytes, void* stream);
 
 /*
+ * Serving operators around the decode step.  None has a counterpart in the
+ * reference, whose runner decodes one greedy token per row and step
+ * (qwen_npu.py:166-236) and prefills one sequence at a time
+ * (prefill_runtime.py:95-164).
+ *
+ * Shared rules: dtype (bf16 or fp16) is the type of q and of every K/V
+ * argument, out_dtype (bf16 or fp16) that of out; strides are in elements,
+ * nonzero multiples of 8; bases are 16-byte aligned; the innermost (head_dim)
+ * axis is contiguous; head_dim 64 or 128; up to 128 q heads per kv head;
+ * scale > 0 multiplies q . k.  lse (may be NULL) is fp32 [rows][n_heads], the
+ * natural log of the softmax sum.  A row that sees no key gets out = 0 and
+ * lse = -inf.  Values of K and V that no row of the call sees may be anything,
+ * infinities and NaN among them.  The lengths, starts and masks are read on
+ * the device; what lies outside the given extents is ignored (clamped), and
+ * output rows that belong to no sequence or to no live node are not written.
+ * The workspace (t2b_varlen_attention_workspace_bytes) needs no
+ * initialisation and is 256-byte aligned; calls that share one must be
+ * ordered on one stream.
+ */
+T2B_API size_t t2b_varlen_attention_workspace_bytes(int rows, int n_heads, int n_kv, int head_dim);
+
+/*
+ * Causal GQA attention over packed sequences of different lengths: query i of
+ * the n = q_start[s+1] - q_start[s] queries of sequence s (rows q_start[s]..
+ * of q and out, total_q rows in all) sees keys 0 .. k_len[s] - n + i of that
+ * sequence:
+ *   out[r, h] = softmax(scale * q[r, h] . K[0..]^T) . V
+ * k_len == n is a whole prompt, k_len > n the last n tokens of a cached one
+ * (n == 1: a decode step).  The sequences' rows are in order and do not
+ * overlap (q_start does not decrease).
+ *   kv_seqs == 0: K and V are packed [kv_tokens][n_kv][head_dim] (strides
+ *     k_tok, k_head, ..); key j of sequence s is row k_start[s] + j.  k_start
+ *     and k_len both NULL: the keys are packed as the queries are.
+ *   kv_seqs >= n_seqs: cache form [kv_seqs][n_kv][kv_tokens][head_dim]
+ *     (strides k_seq, k_head, k_tok, ..); key j of sequence s is row j of
+ *     cache row s.  k_start is NULL, k_len is given.
+ */
+T2B_API int t2b_packed_attention(const void* q, const void* k, const void* v, void* out, float* lse, int dtype,
+                                 int out_dtype, const int32_t* q_start, const int32_t* k_start, const int32_t* k_len,
+                                 int n_seqs, int total_q, int kv_seqs, int kv_tokens, int n_heads, int n_kv,
+                                 int head_dim, size_t q_row, size_t q_head, size_t o_row, size_t o_head, size_t k_tok,
+                                 size_t k_head, size_t k_seq, size_t v_tok, size_t v_head, size_t v_seq, float scale,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * GQA attention of a tree of drafted tokens over the KV cache, T <= 256 nodes
+ * for each of B rows (row b * T + i of q and out is node i of batch row b):
+ * node i sees the ctx_len[b] cached keys of its row and the drafted nodes
+ * j < n_nodes[b] whose bit is set in its mask (bit j % 64 of word j / 64 of
+ * mask[b][i], (T + 63) / 64 words; the node's own bit included).  Caches
+ * [B][n_kv][max_ctx][head_dim], contiguous; the drafted K/V at b * kd_row +
+ * j * kd_node + head * kd_head.  n_nodes NULL: every node is live; nodes from
+ * n_nodes[b] on are not written.
+ */
+T2B_API int t2b_tree_attention(const void* q, const void* k_cache, const void* v_cache, const void* k_draft,
+                               const void* v_draft, void* out, float* lse, int dtype, int out_dtype,
+                               const int32_t* ctx_len, const int32_t* n_nodes, const uint64_t* mask, int B, int T,
+                               int n_heads, int n_kv, int head_dim, int max_ctx, size_t q_row, size_t q_head,
+                               size_t o_row, size_t o_head, size_t kd_row, size_t kd_node, size_t kd_head,
+                               size_t vd_row, size_t vd_node, size_t vd_head, float scale, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
+ * Commit of a verified draft tree.  Row b's walk starts at node 0; from node
+ * c it goes to the lowest node n > c, n < n_nodes[b] (NULL: T), with
+ * parents[b][n] == c and tokens[b][n] == predicted[b][c], as long as the cache
+ * has room.  The i-th node of the walk is path[b][i] (-1 behind its end), its
+ * K/V rows of all n_layers layers (16-bit elements, strides as for
+ * t2b_tree_attention) go to position ctx_len[b] + i of the layers' caches
+ * [B][n_kv][max_ctx][head_dim]; n_accepted[b] is the walk's length,
+ * next_token[b] = predicted[b][last node], new_len[b] = ctx_len[b] +
+ * n_accepted[b].  A row with n_nodes[b] <= 0 or ctx_len[b] outside
+ * [0, max_ctx) accepts nothing (next_token -1, new_len = ctx_len).  Every
+ * other cache row stays as it is.  k_draft .. v_cache are HOST arrays of
+ * n_layers device pointers; drafts and caches must not overlap.
+ */
+T2B_API int t2b_tree_commit(const int32_t* tokens, const int32_t* parents, const int32_t* predicted,
+                            const int32_t* ctx_len, const int32_t* n_nodes, const void* const* k_draft,
+                            const void* const* v_draft, void* const* k_cache, void* const* v_cache, int n_layers,
+                            int32_t* path, int32_t* n_accepted, int32_t* next_token, int32_t* new_len, int B, int T,
+                            int n_kv, int head_dim, int max_ctx, size_t kd_row, size_t kd_node, size_t kd_head,
+                            size_t vd_row, size_t vd_node, size_t vd_head, void* stream);
+
+/*
+ * Log probabilities over logits rows [M][V] (dtype T2B_DTYPE_*, row stride
+ * ld >= V elements), all outputs fp32 and each NULL if not wanted:
+ *   lse[m] = log sum_v exp(x[m, v]);  logprob[m] = x[m, tokens[m]] - lse[m];
+ *   entropy[m] = lse[m] - sum_v p[m, v] x[m, v];
+ *   top_index / top_logprob [M][num_top]: the num_top <= min(32, V) largest
+ *   logits, largest first, ties to the lowest index.
+ * tokens and logprob go together; a token outside [0, V) gets NaN.  -inf
+ * masks a value (p = 0); a row of nothing but -inf gets lse and log
+ * probabilities -inf, entropy 0.  A row with a NaN or +inf gets NaN (NaN
+ * ranks as -inf among the alternatives).
+ */
+T2B_API int t2b_token_logprobs(const void* logits, int dtype, int M, int V, size_t ld, const int32_t* tokens,
+                               float* logprob, float* entropy, float* lse, int num_top, float* top_logprob,
+                               int32_t* top_index, void* stream);
+
+/*
  * Standalone reference operators (same argument meaning as the NPU ops):
  *   RMSNormRoPE (src/torch2iron/operators/rms_norm_rope/op.py:19-90):
  *     out[r] = rope(rmsnorm(in[r]; w, eps), angles[r / (rows/angle_rows)]),

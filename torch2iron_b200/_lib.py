@@ -69,6 +69,13 @@ SIGNATURES = {
     "t2b_lm_head_argmax": (I, [P, P, I, I, I, I, P, P, P, P, Z, P]),
     "t2b_argmax_workspace_bytes": (Z, [I, I]),
     "t2b_argmax_rows": (I, [P, I, I, I, I, P, P, Z, P]),
+    "t2b_varlen_attention_workspace_bytes": (Z, [I, I, I, I]),
+    "t2b_packed_attention": (I, [P, P, P, P, P, I, I, P, P, P, I, I, I, I, I, I, I, Z, Z, Z, Z, Z, Z, Z, Z, Z, Z, F,
+                                 P, Z, P]),
+    "t2b_tree_attention": (I, [P, P, P, P, P, P, P, I, I, P, P, P, I, I, I, I, I, I, Z, Z, Z, Z, Z, Z, Z, Z, Z, Z, F,
+                               P, Z, P]),
+    "t2b_tree_commit": (I, [P, P, P, P, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, Z, Z, Z, Z, Z, Z, P]),
+    "t2b_token_logprobs": (I, [P, I, I, I, Z, P, P, P, P, I, P, P, P]),
     "t2b_rms_norm_rope": (I, [P, P, P, P, I, I, I, F, I, P]),
     "t2b_residual_add_rms_norm": (I, [P, P, P, P, P, I, I, F, P]),
     "t2b_silu_mul": (I, [P, P, P, I, P]),

@@ -18,6 +18,13 @@ Replaced operators (reference file:line):
 * ``SiLUMul``          src/torch2iron/operators/silu_mul/op.py:20-80
 * ``CopyPresentPacketKV``    src/torch2iron/operators/copy_present_packet_kv/op.py:18-80
 
+Operators of a serving loop that the reference has no counterpart for (its
+runner decodes one greedy token per row and step, ``qwen_npu.py:166-236``):
+``PackedAttention`` (causal attention over prompts of different lengths,
+without padding), ``DraftTreeAttention`` and ``DraftTreeCommit`` (verifying a
+tree of drafted tokens over the KV cache and moving the accepted branch into
+it) and ``TokenLogProbs``.
+
 The GEMM family's weight argument is the T2B layout (``W4Weight``) instead
 of the AIE ``aie::mmul<4,8,8>`` tile stream, which has no meaning off the
 NPU; ``W4A16GEMV`` consumes the reference's own ``qparam`` rows unchanged.
@@ -25,13 +32,18 @@ NPU; ``W4A16GEMV`` consumes the reference's own ``qparam`` rows unchanged.
 
 from __future__ import annotations
 
+import ctypes
+import math
 from dataclasses import dataclass, field
 from typing import NamedTuple
 
+import numpy as np
 import torch
 
 from . import _lib
 from .weights import W4Weight
+
+_HALF = (torch.bfloat16, torch.float16)
 
 
 class ArgSpec(NamedTuple):
@@ -399,3 +411,397 @@ class CopyPresentPacketKV:
                   _lib.ptr(packet), self.num_kv_groups, self.head_dim, self.packet_elements_per_group,
                   self.key_packet_offset, self.value_packet_offset, moff, _lib.stream())
         return present_k, present_v, packet
+
+
+# ---------------------------------------------------------------------------
+# serving operators
+# ---------------------------------------------------------------------------
+def _check_arg(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, contiguous: bool = True) -> None:
+    """Shape, type, device and layout of one argument (``shape`` entries of None match anything)."""
+    if tuple(t.shape) != shape and (t.dim() != len(shape) or
+                                    any(want is not None and n != want for n, want in zip(t.shape, shape))):
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: expected a tensor on the current CUDA device, got {t.device}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+
+
+def _strides(name: str, t: torch.Tensor) -> list[int]:
+    """Element strides of every axis but the last (contiguous) one, as the
+    kernels take them: nonzero multiples of 8 on a 16-byte aligned base."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last axis must be contiguous")
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name}: must start on a 16-byte boundary")
+    out = [s if n > 1 else 8 for n, s in zip(t.shape[:-1], t.stride())]    # an axis of one has no stride
+    if any(s % 8 or s <= 0 for s in out):
+        raise ValueError(f"{name}: strides {tuple(t.stride())} must be nonzero multiples of 8 elements")
+    return out
+
+
+def _check_heads(op) -> None:
+    if op.num_kv_groups <= 0:
+        raise ValueError("num_kv_groups must be positive")
+    if not 0 < op.q_heads_per_group <= 128:
+        raise ValueError("q_heads_per_group must be in 1..128")
+    if op.head_dim not in (64, 128):
+        raise ValueError("the B200 kernel needs head_dim in (64, 128)")
+    if op.dtype not in _HALF:
+        raise ValueError("dtype must be torch.bfloat16 or torch.float16")
+    if op.out_dtype is None:
+        op.out_dtype = op.dtype
+    if op.out_dtype not in _HALF:
+        raise ValueError("out_dtype must be torch.bfloat16 or torch.float16")
+    if op.scale is None:
+        op.scale = 1.0 / math.sqrt(op.head_dim)
+    if not (op.scale > 0 and math.isfinite(op.scale)):
+        raise ValueError("scale must be positive and finite")
+
+
+@dataclass
+class PackedAttention:
+    """Causal GQA attention over ``num_seqs`` packed sequences of different lengths.
+
+    ``q`` and ``out`` hold the queries of all sequences one after the other,
+    sequence s in rows ``q_start[s]`` to ``q_start[s + 1] - 1``; query i of its
+    n queries sees keys 0 .. k_len - n + i.  Without ``max_ctx`` the keys are
+    packed ``[kv_tokens, num_kv_groups, head_dim]``, as the queries are or, with
+    ``k_start`` and ``k_len``, from row ``k_start[s]`` on.  With ``max_ctx`` they
+    are cache rows ``[num_seqs, num_kv_groups, max_ctx, head_dim]`` and ``k_len``
+    says how many of each row count, the sequence's own queries among them.
+    A query without keys gets zeros (and ``lse`` -inf); rows of ``out`` and
+    ``lse`` outside every sequence keep what they held."""
+
+    tokens: int
+    num_seqs: int
+    num_kv_groups: int = 8
+    q_heads_per_group: int = 4
+    head_dim: int = 64
+    kv_tokens: int | None = None
+    max_ctx: int | None = None
+    dtype: torch.dtype = torch.bfloat16
+    out_dtype: torch.dtype | None = None
+    scale: float | None = None
+
+    def __post_init__(self):
+        if self.tokens <= 0:
+            raise ValueError("tokens must be positive")
+        if self.num_seqs <= 0:
+            raise ValueError("num_seqs must be positive")
+        if self.max_ctx is not None and (self.max_ctx <= 0 or self.kv_tokens is not None):
+            raise ValueError("max_ctx (cache rows) must be positive and excludes kv_tokens (packed keys)")
+        if self.max_ctx is None and self.kv_tokens is None:
+            self.kv_tokens = self.tokens
+        if self.kv_tokens is not None and self.kv_tokens <= 0:
+            raise ValueError("kv_tokens must be positive")
+        _check_heads(self)
+
+    @property
+    def num_heads(self) -> int:
+        return self.num_kv_groups * self.q_heads_per_group
+
+    def _kv_shape(self) -> tuple:
+        if self.max_ctx is None:
+            return (self.kv_tokens, self.num_kv_groups, self.head_dim)
+        return (self.num_seqs, self.num_kv_groups, self.max_ctx, self.head_dim)
+
+    def get_arg_spec(self):
+        q = (self.tokens, self.num_heads, self.head_dim)
+        return [ArgSpec("in", q, self.dtype), ArgSpec("in", self._kv_shape(), self.dtype),
+                ArgSpec("in", self._kv_shape(), self.dtype), ArgSpec("in", (self.num_seqs + 1,), torch.int32),
+                ArgSpec("out", q, self.out_dtype)]
+
+    def __call__(self, q, k, v, q_start, out, k_start=None, k_len=None, lse=None):
+        for t, spec, nm in zip((q, k, v, q_start, out), self.get_arg_spec(), ("q", "k", "v", "q_start", "out")):
+            _check_arg(nm, t, spec.shape, spec.dtype, contiguous=t is q_start)
+        cached = self.max_ctx is not None
+        if cached and (k_start is not None or k_len is None):
+            raise ValueError("cache rows take k_len and no k_start")
+        if not cached and (k_start is None) != (k_len is None):
+            raise ValueError("packed keys take k_start and k_len together")
+        if not cached and k_start is None and self.kv_tokens != self.tokens:
+            raise ValueError("keys without k_start are packed as the queries are: kv_tokens must equal tokens")
+        for nm, t in (("k_start", k_start), ("k_len", k_len)):
+            if t is not None:
+                _check_arg(nm, t, (self.num_seqs,), torch.int32)
+        if lse is not None:
+            _check_arg("lse", lse, (self.tokens, self.num_heads), torch.float32)
+        qs, os = _strides("q", q), _strides("out", out)
+        ks, vs = _strides("k", k), _strides("v", v)
+        if cached:       # (row, head, token) -> (token, head, row)
+            ks, vs = ks[::-1], vs[::-1]
+        else:
+            ks, vs = ks + [8], vs + [8]
+        L = _lib.lib()
+        n = L.t2b_varlen_attention_workspace_bytes(self.tokens, self.num_heads, self.num_kv_groups, self.head_dim)
+        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+        p = _lib.ptr
+        _lib.check("t2b_packed_attention", L.t2b_packed_attention(
+            p(q), p(k), p(v), p(out), p(lse), _lib.DTYPE[self.dtype], _lib.DTYPE[self.out_dtype], p(q_start),
+            p(k_start), p(k_len), self.num_seqs, self.tokens, self.num_seqs if cached else 0,
+            self.max_ctx if cached else self.kv_tokens, self.num_heads, self.num_kv_groups, self.head_dim, *qs, *os,
+            *ks, *vs, self.scale, p(ws), n, _lib.stream()))
+        return out
+
+
+def draft_tree(parents, num_nodes=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Host helper: ``(mask, depth)`` of drafted trees ``parents [batch, nodes]``.
+
+    Node 0 is the root (its parent entry is not read); every other node's
+    parent precedes it.  ``mask`` int64 ``[batch, nodes, (nodes + 63) // 64]``
+    has the bits of each node's ancestors and of the node itself, ``depth``
+    int32 ``[batch, nodes]`` its distance from the root.  Nodes from
+    ``num_nodes[b]`` on get an empty mask and depth 0."""
+    par = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
+    if par.ndim != 2 or par.shape[1] < 1 or not np.issubdtype(par.dtype, np.integer):
+        raise ValueError("parents must be integers [batch, nodes]")
+    B, T = par.shape
+    live = np.full(B, T) if num_nodes is None else \
+        np.asarray(num_nodes.cpu() if isinstance(num_nodes, torch.Tensor) else num_nodes).reshape(-1)
+    if live.shape != (B,) or live.min(initial=0) < 0 or live.max(initial=0) > T:
+        raise ValueError(f"num_nodes must be {B} values in 0..{T}")
+    node = np.arange(T)
+    used = node[None] < live[:, None]
+    if (used & (node[None] > 0) & ((par < 0) | (par >= node[None]))).any():
+        raise ValueError("a node's parent must precede it")
+    sees = np.zeros((B, T, T), bool)
+    depth = np.zeros((B, T), np.int32)
+    rows = np.arange(B)
+    for i in range(T):
+        if i:
+            up = np.where(used[:, i], par[:, i], 0)
+            sees[:, i] = sees[rows, up]
+            depth[:, i] = depth[rows, up] + 1
+        sees[:, i, i] = True
+        sees[~used[:, i], i] = False
+        depth[~used[:, i], i] = 0
+    words = (T + 63) // 64
+    bits = np.zeros((B, T, words * 64), np.uint8)
+    bits[:, :, :T] = sees
+    packed = np.packbits(bits, axis=2, bitorder="little")
+    return torch.from_numpy(packed.view("<i8").reshape(B, T, words).copy()), torch.from_numpy(depth)
+
+
+@dataclass
+class DraftTreeAttention:
+    """GQA attention of ``nodes`` drafted tokens per batch row over the KV cache.
+
+    Node i of row b sees the ``ctx_len[b]`` cached keys of its row and the
+    drafted nodes whose bit is set in ``mask[b, i]`` (``draft_tree``); the
+    drafted K/V stay outside the cache until ``DraftTreeCommit`` moves the
+    accepted ones.  Nodes from ``num_nodes[b]`` on are not computed: their rows
+    of ``out`` and ``lse`` keep what they held."""
+
+    batch: int
+    nodes: int
+    max_ctx: int
+    num_kv_groups: int = 8
+    q_heads_per_group: int = 4
+    head_dim: int = 64
+    dtype: torch.dtype = torch.bfloat16
+    out_dtype: torch.dtype | None = None
+    scale: float | None = None
+
+    def __post_init__(self):
+        if self.batch <= 0:
+            raise ValueError("batch must be positive")
+        if not 0 < self.nodes <= 256:
+            raise ValueError("the B200 kernel needs nodes in 1..256")
+        if self.max_ctx <= 0:
+            raise ValueError("max_ctx must be positive")
+        _check_heads(self)
+
+    @property
+    def num_heads(self) -> int:
+        return self.num_kv_groups * self.q_heads_per_group
+
+    @property
+    def mask_words(self) -> int:
+        return (self.nodes + 63) // 64
+
+    def get_arg_spec(self):
+        q = (self.batch, self.nodes, self.num_heads, self.head_dim)
+        cache = (self.batch, self.num_kv_groups, self.max_ctx, self.head_dim)
+        draft = (self.batch, self.nodes, self.num_kv_groups, self.head_dim)
+        return [ArgSpec("in", q, self.dtype), ArgSpec("in", cache, self.dtype), ArgSpec("in", cache, self.dtype),
+                ArgSpec("in", draft, self.dtype), ArgSpec("in", draft, self.dtype),
+                ArgSpec("in", (self.batch,), torch.int32),
+                ArgSpec("in", (self.batch, self.nodes, self.mask_words), torch.int64), ArgSpec("out", q, self.out_dtype)]
+
+    def __call__(self, q, k_cache, v_cache, k_draft, v_draft, ctx_len, mask, out, num_nodes=None, lse=None):
+        names = ("q", "k_cache", "v_cache", "k_draft", "v_draft", "ctx_len", "mask", "out")
+        for t, spec, nm in zip((q, k_cache, v_cache, k_draft, v_draft, ctx_len, mask, out), self.get_arg_spec(), names):
+            _check_arg(nm, t, spec.shape, spec.dtype, contiguous=nm in ("k_cache", "v_cache", "ctx_len", "mask"))
+        if num_nodes is not None:
+            _check_arg("num_nodes", num_nodes, (self.batch,), torch.int32)
+        if lse is not None:
+            _check_arg("lse", lse, (self.batch, self.nodes, self.num_heads), torch.float32)
+        qs, os = self._rows("q", q), self._rows("out", out)
+        kd, vd = _strides("k_draft", k_draft), _strides("v_draft", v_draft)
+        _strides("k_cache", k_cache), _strides("v_cache", v_cache)
+        L = _lib.lib()
+        n = L.t2b_varlen_attention_workspace_bytes(self.batch * self.nodes, self.num_heads, self.num_kv_groups,
+                                                   self.head_dim)
+        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+        p = _lib.ptr
+        _lib.check("t2b_tree_attention", L.t2b_tree_attention(
+            p(q), p(k_cache), p(v_cache), p(k_draft), p(v_draft), p(out), p(lse), _lib.DTYPE[self.dtype],
+            _lib.DTYPE[self.out_dtype], p(ctx_len), p(num_nodes), p(mask), self.batch, self.nodes, self.num_heads,
+            self.num_kv_groups, self.head_dim, self.max_ctx, *qs, *os, *kd, *vd, self.scale, p(ws), n, _lib.stream()))
+        return out
+
+    def _rows(self, name, t) -> list[int]:
+        """(row, head) strides of ``[batch, nodes, ..]`` seen as ``[batch * nodes, ..]``."""
+        b, node, head = _strides(name, t)
+        if self.nodes == 1:
+            return [b, head]
+        if self.batch > 1 and b != self.nodes * node:
+            raise ValueError(f"{name}: the nodes of consecutive batch rows must follow one another")
+        return [node, head]
+
+
+@dataclass
+class DraftTreeCommit:
+    """Greedy walk through each row's verified tree, and the move of the
+    accepted nodes' K/V rows of every layer into the caches.
+
+    From node c the walk goes to the lowest later node n with ``parents[n] ==
+    c`` and ``tokens[n] == predicted[c]`` (``predicted``: the model's token
+    after each node), while the cache has room.  ``k_drafts`` / ``v_drafts``
+    are ``[layers, batch, nodes, kv, head_dim]`` or a sequence of one tensor per
+    layer, ``k_caches`` / ``v_caches`` likewise ``[layers, batch, kv, max_ctx,
+    head_dim]``.  Writes ``path`` (-1 behind the walk's end), ``num_accepted``,
+    ``next_token`` and ``new_len = ctx_len + num_accepted``; a row with no live
+    node or no room accepts nothing (next token -1)."""
+
+    layers: int
+    batch: int
+    nodes: int
+    max_ctx: int
+    num_kv_groups: int = 8
+    head_dim: int = 64
+    dtype: torch.dtype = torch.bfloat16
+
+    def __post_init__(self):
+        if self.layers <= 0 or self.batch <= 0:
+            raise ValueError("layers and batch must be positive")
+        if not 0 < self.nodes <= 256:
+            raise ValueError("the B200 kernel needs nodes in 1..256")
+        if self.max_ctx <= 0:
+            raise ValueError("max_ctx must be positive")
+        if not 0 < self.num_kv_groups <= 1024:
+            raise ValueError("num_kv_groups must be in 1..1024")
+        if self.head_dim <= 0 or self.head_dim % 8 or self.head_dim > 1024:
+            raise ValueError("head_dim must be a multiple of 8, at most 1024")
+        if self.dtype not in _HALF:
+            raise ValueError("dtype must be torch.bfloat16 or torch.float16")
+
+    def get_arg_spec(self):
+        i32, tree = torch.int32, (self.batch, self.nodes)
+        draft = (self.layers, self.batch, self.nodes, self.num_kv_groups, self.head_dim)
+        cache = (self.layers, self.batch, self.num_kv_groups, self.max_ctx, self.head_dim)
+        return [ArgSpec("in", tree, i32), ArgSpec("in", tree, i32), ArgSpec("in", tree, i32),
+                ArgSpec("in", (self.batch,), i32), ArgSpec("in", draft, self.dtype), ArgSpec("in", draft, self.dtype),
+                ArgSpec("inout", cache, self.dtype), ArgSpec("inout", cache, self.dtype), ArgSpec("out", tree, i32),
+                ArgSpec("out", (self.batch,), i32), ArgSpec("out", (self.batch,), i32),
+                ArgSpec("out", (self.batch,), i32)]
+
+    def _layers(self, name: str, ts, shape: tuple, contiguous: bool):
+        """Host array of the layers' device pointers, and the strides they share."""
+        if isinstance(ts, torch.Tensor):
+            _check_arg(name, ts, (self.layers, *shape), self.dtype, contiguous=False)
+            one, step = ts[0], ts.stride(0) * ts.element_size()
+            at = [ts.data_ptr() + i * step for i in range(self.layers)]
+        else:
+            if len(ts) != self.layers:
+                raise ValueError(f"{name}: expected {self.layers} layers, got {len(ts)}")
+            one = ts[0]
+            for t in ts:
+                _check_arg(name, t, shape, self.dtype, contiguous=False)
+                if t.stride() != one.stride():
+                    raise ValueError(f"{name}: the layers' strides differ")
+            at = [t.data_ptr() for t in ts]
+        if contiguous and not one.is_contiguous():
+            raise ValueError(f"{name}: must be contiguous")
+        strides = _strides(name, one)
+        if any(a % 16 for a in at):
+            raise ValueError(f"{name}: must start on a 16-byte boundary")
+        return (ctypes.c_void_p * self.layers)(*at), strides
+
+    def __call__(self, tokens, parents, predicted, ctx_len, k_drafts, v_drafts, k_caches, v_caches, path, num_accepted,
+                 next_token, new_len, num_nodes=None):
+        i32, tree, row = torch.int32, (self.batch, self.nodes), (self.batch,)
+        for nm, t, shape in (("tokens", tokens, tree), ("parents", parents, tree), ("predicted", predicted, tree),
+                             ("ctx_len", ctx_len, row), ("path", path, tree), ("num_accepted", num_accepted, row),
+                             ("next_token", next_token, row), ("new_len", new_len, row)):
+            _check_arg(nm, t, shape, i32)
+        if num_nodes is not None:
+            _check_arg("num_nodes", num_nodes, row, i32)
+        draft = (self.batch, self.nodes, self.num_kv_groups, self.head_dim)
+        cache = (self.batch, self.num_kv_groups, self.max_ctx, self.head_dim)
+        kd, kds = self._layers("k_drafts", k_drafts, draft, False)
+        vd, vds = self._layers("v_drafts", v_drafts, draft, False)
+        kc, _ = self._layers("k_caches", k_caches, cache, True)
+        vc, _ = self._layers("v_caches", v_caches, cache, True)
+        p = _lib.ptr
+        _lib.call("t2b_tree_commit", p(tokens), p(parents), p(predicted), p(ctx_len), p(num_nodes), kd, vd, kc, vc,
+                  self.layers, p(path), p(num_accepted), p(next_token), p(new_len), self.batch, self.nodes,
+                  self.num_kv_groups, self.head_dim, self.max_ctx, *kds, *vds, _lib.stream())
+        return path, num_accepted, next_token, new_len
+
+
+@dataclass
+class TokenLogProbs:
+    """Log probabilities of given tokens over logits rows, with the entropy and
+    the ``num_top`` most likely tokens of each row (largest first, ties to the
+    lowest index), in fp32.
+
+    ``logits [rows, vocab]`` may have a row stride above ``vocab``.  A token
+    outside the vocabulary gets NaN; a value of -inf is masked out, and a row of
+    nothing else gets log probabilities -inf and entropy 0."""
+
+    rows: int
+    vocab: int
+    num_top: int = 0
+    dtype: torch.dtype = torch.float32
+
+    def __post_init__(self):
+        if self.rows <= 0 or self.vocab <= 0:
+            raise ValueError("rows and vocab must be positive")
+        if not 0 <= self.num_top <= min(32, self.vocab):
+            raise ValueError("num_top must be in 0..min(32, vocab)")
+        if self.dtype not in _lib.DTYPE:
+            raise ValueError("dtype must be torch.float32, torch.bfloat16 or torch.float16")
+
+    def get_arg_spec(self):
+        f32, row = torch.float32, (self.rows,)
+        spec = [ArgSpec("in", (self.rows, self.vocab), self.dtype), ArgSpec("in", row, torch.int32),
+                ArgSpec("out", row, f32), ArgSpec("out", row, f32)]
+        if self.num_top:
+            spec += [ArgSpec("out", (self.rows, self.num_top), f32),
+                     ArgSpec("out", (self.rows, self.num_top), torch.int32)]
+        return spec
+
+    def __call__(self, logits, tokens, logprob, entropy=None, top_logprob=None, top_index=None, lse=None):
+        f32 = torch.float32
+        _check_arg("logits", logits, (self.rows, self.vocab), self.dtype, contiguous=False)
+        if self.vocab > 1 and logits.stride(1) != 1 or self.rows > 1 and logits.stride(0) < self.vocab:
+            raise ValueError("logits: rows must be contiguous and must not overlap")
+        _check_arg("tokens", tokens, (self.rows,), torch.int32)
+        _check_arg("logprob", logprob, (self.rows,), f32)
+        for nm, t in (("entropy", entropy), ("lse", lse)):
+            if t is not None:
+                _check_arg(nm, t, (self.rows,), f32)
+        if (self.num_top > 0) != (top_logprob is not None) or (self.num_top > 0) != (top_index is not None):
+            raise ValueError("top_logprob and top_index go with num_top > 0")
+        if self.num_top:
+            _check_arg("top_logprob", top_logprob, (self.rows, self.num_top), f32)
+            _check_arg("top_index", top_index, (self.rows, self.num_top), torch.int32)
+        p = _lib.ptr
+        _lib.call("t2b_token_logprobs", p(logits), _lib.DTYPE[self.dtype], self.rows, self.vocab,
+                  logits.stride(0) if self.rows > 1 else self.vocab, p(tokens), p(logprob), p(entropy), p(lse),
+                  self.num_top, p(top_logprob), p(top_index), _lib.stream())
+        return logprob
