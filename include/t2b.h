@@ -429,7 +429,7 @@ T2B_API int t2b_argmax_rows(const void* logits, int dtype, int M, int V, int ld,
  * initialisation and is 256-byte aligned; calls that share one must be
  * ordered on one stream.
  */
-T2B_API size_t t2b_varlen_attention_workspace_bytes(int rows, int n_heads, int n_kv, int head_dim);
+T2B_API size_t t2b_varlen_attention_workspace_bytes(int head_dim);
 
 /*
  * Causal GQA attention over packed sequences of different lengths: query i of

@@ -69,7 +69,7 @@ SIGNATURES = {
     "t2b_lm_head_argmax": (I, [P, P, I, I, I, I, P, P, P, P, Z, P]),
     "t2b_argmax_workspace_bytes": (Z, [I, I]),
     "t2b_argmax_rows": (I, [P, I, I, I, I, P, P, Z, P]),
-    "t2b_varlen_attention_workspace_bytes": (Z, [I, I, I, I]),
+    "t2b_varlen_attention_workspace_bytes": (Z, [I]),
     "t2b_packed_attention": (I, [P, P, P, P, P, I, I, P, P, P, I, I, I, I, I, I, I, Z, Z, Z, Z, Z, Z, Z, Z, Z, Z, F,
                                  P, Z, P]),
     "t2b_tree_attention": (I, [P, P, P, P, P, P, P, I, I, P, P, P, I, I, I, I, I, I, Z, Z, Z, Z, Z, Z, Z, Z, Z, Z, F,

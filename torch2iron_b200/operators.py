@@ -536,8 +536,8 @@ class PackedAttention:
         else:
             ks, vs = ks + [8], vs + [8]
         L = _lib.lib()
-        n = L.t2b_varlen_attention_workspace_bytes(self.tokens, self.num_heads, self.num_kv_groups, self.head_dim)
-        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+        n = L.t2b_varlen_attention_workspace_bytes(self.head_dim)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         p = _lib.ptr
         _lib.check("t2b_packed_attention", L.t2b_packed_attention(
             p(q), p(k), p(v), p(out), p(lse), _lib.DTYPE[self.dtype], _lib.DTYPE[self.out_dtype], p(q_start),
@@ -643,9 +643,8 @@ class DraftTreeAttention:
         kd, vd = _strides("k_draft", k_draft), _strides("v_draft", v_draft)
         _strides("k_cache", k_cache), _strides("v_cache", v_cache)
         L = _lib.lib()
-        n = L.t2b_varlen_attention_workspace_bytes(self.batch * self.nodes, self.num_heads, self.num_kv_groups,
-                                                   self.head_dim)
-        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+        n = L.t2b_varlen_attention_workspace_bytes(self.head_dim)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         p = _lib.ptr
         _lib.check("t2b_tree_attention", L.t2b_tree_attention(
             p(q), p(k_cache), p(v_cache), p(k_draft), p(v_draft), p(out), p(lse), _lib.DTYPE[self.dtype],
