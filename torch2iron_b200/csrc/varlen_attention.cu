@@ -54,13 +54,14 @@ namespace t2b {
 
 constexpr int VA_MAX_NODES = 256;
 constexpr int VA_ROWS = 128;            // rows per tile (MMA M), keys per block (MMA N)
-constexpr int VA_THREADS = 384;         // 8 softmax warps, TMA, MMA, 2 that only fill the warpgroup
-// Registers: 384 threads are launched with 168 each (64512); the softmax
-// warpgroups take 208 and the third gives down to 80: 2 * 128 * 208 + 128 * 80
-// = 63488.
-constexpr int VA_REGS_SOFTMAX = 208, VA_REGS_OTHER = 80;
-constexpr int VA_SNAP = 4;              // items of up to this many blocks stay in one CTA
-constexpr int VA_MIN_UNITS = 2;         // units per CTA, at least
+constexpr int VA_THREADS = 640;         // 16 softmax warps, TMA, MMA, 2 that only fill the warpgroup
+// Registers: 640 threads are launched with 96 each (61440); the four softmax
+// warpgroups take 104 and the fifth gives down to 64: 512 * 104 + 128 * 64 = 61440.
+constexpr int VA_REGS_SOFTMAX = 104, VA_REGS_OTHER = 64;
+constexpr int VA_WARP_TMA = 16, VA_WARP_MMA = 17;
+constexpr int VA_ITEM = 2;              // what an item costs beside its blocks, in blocks (see Work)
+constexpr int VA_SNAP = 8;              // items of up to this many blocks stay in one CTA
+constexpr int VA_MIN_UNITS = 3;         // units per CTA, at least
 constexpr float VA_HEAD = 7.f, VA_ROOM = 15.f;
 
 struct VaParams {
@@ -91,10 +92,11 @@ struct VaGeom {
   static constexpr int STAGES = HD == 128 ? 5 : 8;     // K and V blocks in flight
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_ML = OFF_KV + STAGES * TILE;   // float2 [128]: group 1's (m, l)
-  static constexpr int OFF_BAR = OFF_ML + VA_ROWS * 8;
-  static constexpr int N_BARS = 2 + 2 * STAGES + 9;
+  static constexpr int OFF_X = OFF_ML + VA_ROWS * 8;      // float [2][128]: what the halves of a row tell each other
+  static constexpr int OFF_BAR = OFF_X + 2 * VA_ROWS * 4;
+  static constexpr int N_BARS = 2 + 2 * STAGES + 11;
   static constexpr int OFF_MISC = OFF_BAR + N_BARS * 8;
-  static constexpr int BYTES = OFF_MISC + 256 + 1024;      // + slack to 1024-align the base
+  static constexpr int BYTES = OFF_MISC + 192;
   static constexpr uint32_t S0 = 0, O0 = 256;              // TMEM columns: S_t at S0 + 128 t, O_t at O0 + HD t
   static_assert(BYTES <= 232448, "shared memory of one CTA");
 };
@@ -134,51 +136,81 @@ T2B_DEV int va_tile_blocks(const VaSeq& q, int tpt, int p, int t) {
   if (TREE) return va_blocks(q.avail) + va_blocks(q.n);
   return max(1, va_blocks(va_limit(q, min(q.n, (2 * p + t + 1) * tpt) - 1)));
 }
-T2B_DEV int va_pairs(const VaSeq& q, int tpt) { return (q.n + 2 * tpt - 1) / (2 * tpt); }
+// x / t for x >= 0; a shift where t is a power of two (as the q heads per kv head mostly are)
+T2B_DEV int va_div(int x, int t) { return (t & (t - 1)) == 0 ? x >> (__ffs(t) - 1) : x / t; }
+T2B_DEV int va_pairs(const VaSeq& q, int tpt) { return va_div(q.n + 2 * tpt - 1, 2 * tpt); }
+// sum of floor((a i + b) / 128), i < n, by the Euclidean recursion on the
+// lattice points under a line (its divisions are by 128, by a, ..).
+T2B_DEV uint32_t va_floor_sum(uint32_t n, uint32_t a, uint32_t b) {
+  uint32_t sum = 0, m = VA_ROWS;
+  while (n) {
+    const uint32_t qa = va_div(a, m), qb = va_div(b, m);
+    sum += n * (n - 1) / 2 * qa + n * qb;
+    a -= qa * m;
+    b -= qb * m;
+    const uint32_t y = a * n + b;
+    n = va_div(y, m);
+    b = y - n * m;
+    const uint32_t t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+// Blocks of pairs 0 .. k - 1 of a sequence, in closed form: pairs that see at
+// most one block, then a line's blocks, then pairs that see every key.  (The
+// sequences of a long prompt have hundreds of pairs; a loop over them cost
+// 14 us at the start of a 1.9 ms call.)
+template <bool TREE>
+T2B_DEV uint32_t va_blocks_before(const VaSeq& q, int tpt, int pairs, int k) {
+  if (TREE) return k ? (uint32_t)k * va_tile_blocks<TREE>(q, tpt, 0, 0) : 0u;
+  uint32_t sum = 0;
+  if (k == pairs && k > 0) sum = va_tile_blocks<TREE>(q, tpt, --k, 1);   // the last pair may be short
+  const int t = 2 * tpt;                                // pair p sees min(off + (p + 1) t, avail) keys
+  const int one = VA_ROWS - q.off < t ? 0 : min(k, va_div(VA_ROWS - q.off, t));
+  const int rise = q.avail - q.off <= 0 ? one : max(one, min(k, va_div(q.avail - q.off + t - 1, t) - 1));
+  sum += one + (k - rise) * max(1, va_blocks(q.avail));
+  if (rise > one) sum += va_floor_sum(rise - one, t, q.off + (one + 1) * t + VA_ROWS - 1);
+  return sum;
+}
 
 // A position in the list of units: block b of item (s, p, g).
 struct VaCursor {
   int s, p, g, b;
 };
-struct VaSegment {
-  VaSeq q;
-  int s, p, g;
-  int b0, n;          // first block, blocks of this CTA
-  int nb, n0;         // the item's blocks; blocks of tile 0 in this segment (two tiles)
-  bool dual;          // both tiles live
-};
-
+// Walks a range of the list, one item's blocks at a time.
 template <bool TREE>
 struct VaWalk {
-  VaCursor c;
-  int left;
-  VaSeq q;
-  T2B_DEV VaWalk(const VaParams& P, VaCursor at, int units) : c(at), left(units) {
-    if (left > 0) q = va_seq<TREE>(P, c.s);
-  }
-  T2B_DEV bool next(const VaParams& P, VaSegment& seg) {
+  VaSeq q;            // the item's sequence
+  int s, p, g;        // the item
+  int b0, n;          // first block, blocks of this CTA
+  int nb, n0;         // the item's blocks; blocks of tile 0 among the n (two tiles)
+  bool dual;          // both tiles live
+  int left;           // units behind this item's
+
+  T2B_DEV VaWalk(VaCursor at, int units) : s(at.s), p(at.p), g(at.g - 1), b0(at.b), n(-1), left(units) {}
+  T2B_DEV bool next(const VaParams& P) {
     if (left <= 0) return false;
-    seg.q = q;
-    seg.s = c.s;
-    seg.p = c.p;
-    seg.g = c.g;
-    seg.dual = q.n > (2 * c.p + 1) * P.tpt;
-    seg.nb = va_tile_blocks<TREE>(q, P.tpt, c.p, seg.dual ? 1 : 0);
-    seg.b0 = c.b;
-    seg.n = min(left, seg.nb - c.b);
-    seg.n0 = seg.dual ? min(seg.n, va_tile_blocks<TREE>(q, P.tpt, c.p, 0) - c.b) : seg.n;
-    left -= seg.n;
-    c.b = 0;
-    if (left > 0 && ++c.g == P.n_kv) {
-      c.g = 0;
-      if (++c.p == va_pairs(q, P.tpt)) {
-        c.p = 0;
+    if (n < 0) {
+      q = va_seq<TREE>(P, s);
+    } else {
+      b0 = 0;
+    }
+    if (++g == P.n_kv) {
+      g = 0;
+      if (++p == va_pairs(q, P.tpt)) {
+        p = 0;
         do {
-          ++c.s;
-          q = va_seq<TREE>(P, c.s);
-        } while (q.n == 0 && c.s + 1 < P.n_seqs);
+          ++s;
+          q = va_seq<TREE>(P, s);
+        } while (q.n == 0 && s + 1 < P.n_seqs);
       }
     }
+    dual = q.n > (2 * p + 1) * P.tpt;
+    nb = va_tile_blocks<TREE>(q, P.tpt, p, dual ? 1 : 0);
+    n = min(left, nb - b0);
+    n0 = dual ? min(n, va_tile_blocks<TREE>(q, P.tpt, p, 0) - b0) : n;
+    left -= n + (b0 + n == nb ? VA_ITEM : 0);
     return true;
   }
 };
@@ -189,6 +221,9 @@ T2B_DEV void tma_load_4d(void* dst, const void* tmap, int x, int y, int z, int w
       "[%6];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
+}
+T2B_DEV void va_prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 // UMMA descriptor of an MN-major operand, 128-byte swizzle: 64 contiguous
 // elements per 128-byte row, 8-row groups 1024 B apart along k, the next 64
@@ -212,6 +247,38 @@ T2B_DEV void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+// One lane of the (converged) warp.  The MMAs are issued under this predicate
+// and not under lane == 0: ptxas then knows that one lane runs the block and
+// keeps the descriptors in uniform registers (64 clocks per 128x128x16 MMA,
+// the pipe's rate, against 134 to issue one under a lane test).
+T2B_DEV bool va_elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// two fp32 values in one 64-bit register: the packed forms issue both lanes at once
+typedef unsigned long long f32x2;
+T2B_DEV f32x2 va_pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+T2B_DEV void va_split(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+T2B_DEV f32x2 va_fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+T2B_DEV f32x2 va_add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+T2B_DEV float va_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 T2B_DEV float va_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -226,6 +293,56 @@ T2B_DEV uint32_t va_pack(float lo, float hi) {
 }
 T2B_DEV uint32_t va_pack_out(float lo, float hi, int f16) { return f16 ? f16x2_sat(lo, hi) : va_pack<false>(lo, hi); }
 
+// The whole warp waits for a phase of `bar`, at most 0.5 s: true once it is
+// complete, false (the same in every lane) when the time is up or another role
+// of the CTA has given up.
+T2B_DEV bool va_wait(uint64_t* bar, uint32_t phase, volatile int* abort_flag, int* err) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) return true;
+    const bool late = globaltimer_ns() - t0 > 500000000ull;
+    if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
+      if (late && err) atomicCAS(err, 0, T2B_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+// The two warps that hold the halves of 32 rows: a barrier, and one that
+// returns whether any of their 64 lanes says so.
+T2B_DEV void va_pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+T2B_DEV bool va_pair_any(int id, bool v) {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(r)
+               : "r"((uint32_t)v), "r"(id)
+               : "memory");
+  return r != 0;
+}
+
+// 4x4 transpose of 16-byte pieces over a quad of lanes.
+T2B_DEV void va_transpose(uint4 (&x)[4], int lane) {
+#pragma unroll
+  for (int m = 1; m <= 2; m <<= 1) {
+    const bool up = (lane & m) != 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (c & m) continue;
+      const uint4 send = up ? x[c] : x[c + m];
+      uint4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, send.x, m);
+      got.y = __shfl_xor_sync(0xffffffffu, send.y, m);
+      got.z = __shfl_xor_sync(0xffffffffu, send.z, m);
+      got.w = __shfl_xor_sync(0xffffffffu, send.w, m);
+      if (up) x[c] = got;
+      else x[c + m] = got;
+    }
+  }
+}
+
 // Keys 32 w .. 32 w + 31 below `n` of a block, as bits.
 T2B_DEV uint32_t va_bits_below(int n, int w) {
   const int k = n - 32 * w;
@@ -237,26 +354,37 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
   using G = VaGeom<HD>;
   constexpr int NS = G::STAGES, HALVES = HD / 64;
   extern __shared__ __align__(1024) uint8_t smem_dyn[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  uint8_t* sm = smem_dyn;
+  if (smem_u32(sm) & 1023) {   // (the swizzled tiles need it; the kernel has no other shared memory)
+    if (threadIdx.x == 0) {
+      P.head[2 * blockIdx.x] = P.head[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
+      if (P.err) atomicCAS(P.err, 0, T2B_ERR_ALIGN);
+    }
+    return;
+  }
+  float* s_x = reinterpret_cast<float*>(sm + G::OFF_X);
   float2* s_ml = reinterpret_cast<float2*>(sm + G::OFF_ML);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(sm + G::OFF_BAR);
   uint64_t* q_empty = q_full + 1;
   uint64_t* kv_full = q_full + 2;
   uint64_t* kv_empty = kv_full + NS;
   uint64_t* s_full = kv_empty + NS;      // [2]
-  uint64_t* p_full = s_full + 2;         // [2]
-  uint64_t* o_full = p_full + 2;         // [2]
+  uint64_t* p_full = s_full + 2;         // [2][halves of a block]
+  uint64_t* o_full = p_full + 4;         // [2]
   uint64_t* g1_full = o_full + 2;
   uint64_t* g1_empty = g1_full + 1;
   uint64_t* done = g1_full + 2;
-  long long* s_scan = reinterpret_cast<long long*>(sm + G::OFF_MISC);          // [11]
-  VaCursor* s_at = reinterpret_cast<VaCursor*>(sm + G::OFF_MISC + 96);
-  int* s_flag = reinterpret_cast<int*>(sm + G::OFF_MISC + 128);
-  long long* s_range = reinterpret_cast<long long*>(sm + G::OFF_MISC + 144);   // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC + 160);
+  uint32_t* s_scan = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC);            // [warps]
+  VaCursor* s_at = reinterpret_cast<VaCursor*>(sm + G::OFF_MISC + 80);
+  uint2* s_cut = reinterpret_cast<uint2*>(sm + G::OFF_MISC + 96);              // [2]: sequence, unit inside it
+  uint32_t* s_range = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC + 112);     // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + G::OFF_MISC + 120);
+  int* s_flag = reinterpret_cast<int*>(sm + G::OFF_MISC + 124);
+  volatile int* s_bad = reinterpret_cast<volatile int*>(sm + G::OFF_MISC + 128);   // [8]: a warp of the pair gave up
   volatile int* abort_flag = s_flag;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // (uniform, and known to be)
   if (tid == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -266,111 +394,132 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);   // one arrival per softmax warp
+      mbar_init(&p_full[2 * t], 4);   // one arrival per softmax warp
+      mbar_init(&p_full[2 * t + 1], 4);
       mbar_init(&o_full[t], 1);
     }
-    mbar_init(g1_full, 4);
-    mbar_init(g1_empty, 4);
+    mbar_init(g1_full, 8);    // one arrival per warp of the group
+    mbar_init(g1_empty, 8);
     mbar_init(done, 1);
     *abort_flag = 0;
+    for (int i = 0; i < 8; ++i) s_bad[i] = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (tid == 32) {   // the descriptors are kernel parameters: their fetch need not wait for the predecessor
+    va_prefetch_map(&P.qmap);
+    va_prefetch_map(&P.kmap);
+    va_prefetch_map(&P.vmap);
+    if (TREE) {
+      va_prefetch_map(&P.kdmap);
+      va_prefetch_map(&P.vdmap);
+    }
+  }
+  if (warp == VA_WARP_MMA) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   grid_dep_wait();
 
-  // ---- this CTA's range of the list of units ----
+  // ---- this CTA's range of the list of units (at most 2^31 - 1: checked on the host) ----
   const int c = blockIdx.x;
-  auto seq_units = [&](int s) -> long long {
+  VaSeq mine;
+  auto seq_units = [&](int s) -> uint32_t {
     if (s >= P.n_seqs) return 0;
-    const VaSeq q = va_seq<TREE>(P, s);
-    const int pairs = va_pairs(q, P.tpt);
-    long long u = 0;
-    if (TREE) {
-      u = (long long)pairs * va_tile_blocks<TREE>(q, P.tpt, 0, 0);
-    } else {
-      for (int p = 0; p < pairs; ++p) u += va_tile_blocks<TREE>(q, P.tpt, p, 1);
-    }
-    return u * P.n_kv;
+    mine = va_seq<TREE>(P, s);
+    const int pairs = va_pairs(mine, P.tpt);
+    return (va_blocks_before<TREE>(mine, P.tpt, pairs, pairs) + pairs * VA_ITEM) * P.n_kv;
   };
-  // inclusive sum of one value per thread over the block (and the block's total)
-  auto block_scan = [&](long long v, long long& total) -> long long {
+  // inclusive sum of one value per thread over the block, and the block's total
+  auto block_scan = [&](uint32_t v, uint32_t& sum) -> uint32_t {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long w = __shfl_up_sync(0xffffffffu, v, o);
+      const uint32_t w = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += w;
     }
     __syncthreads();
     if (lane == 31) s_scan[warp] = v;
     __syncthreads();
-    long long before = 0;
-    total = 0;
+    uint32_t before = 0;
+    sum = 0;
+#pragma unroll
     for (int w = 0; w < VA_THREADS / 32; ++w) {
-      if (w < warp) before += s_scan[w];
-      total += s_scan[w];
+      const uint32_t x = s_scan[w];
+      before += w < warp ? x : 0u;
+      sum += x;
     }
     return before + v;
   };
-  long long total = 0;
+  uint32_t total = 0, units0 = 0, end0 = 0;   // the first VA_THREADS sequences' are kept
   for (int s0 = 0; s0 < P.n_seqs; s0 += VA_THREADS) {
-    long long t;
-    block_scan(seq_units(s0 + tid), t);
-    total += t;
+    uint32_t sum;
+    const uint32_t u = seq_units(s0 + tid), e = block_scan(u, sum);
+    if (s0 == 0) units0 = u, end0 = e;
+    total += sum;
   }
-  const int parts = (int)min((long long)gridDim.x, max(1ll, total / VA_MIN_UNITS));
-  const bool busy = total > 0 && c < parts;
+  const uint32_t parts = min((uint32_t)gridDim.x, max(1u, total / VA_MIN_UNITS));
+  const bool busy = total > 0 && c < (int)parts;
+  const uint32_t each = total / parts, more = total - each * parts;   // the first `more` ranges have one unit more
+  const uint32_t cut[2] = {each * c + min((uint32_t)c, more), each * (c + 1) + min((uint32_t)c + 1, more)};
   if (tid == 0) {
     s_range[0] = 0;
     s_range[1] = busy ? total : 0;   // (kept where the range's end is the end of the list)
+    s_cut[0] = s_cut[1] = make_uint2(0xffffffffu, 0u);
   }
   if (busy) {
-    const long long cut[2] = {total * c / parts, total * (c + 1) / parts};
-    long long base = 0;
+    uint32_t base = 0;
     for (int s0 = 0; s0 < P.n_seqs; s0 += VA_THREADS) {
-      long long t;
-      const long long mine = seq_units(s0 + tid);
-      const long long end = base + block_scan(mine, t), begin = end - mine;
-      base += t;
+      uint32_t u = units0, e = end0, sum;
+      if (P.n_seqs > VA_THREADS) {
+        u = seq_units(s0 + tid);
+        e = block_scan(u, sum) + base;
+        base += sum;
+      } else {
+        __syncthreads();
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (cut[i] >= begin && cut[i] < end) {   // the cut falls into sequence s0 + tid
-          const int s = s0 + tid;
-          const VaSeq q = va_seq<TREE>(P, s);
-          const int pairs = va_pairs(q, P.tpt);
-          long long u = begin;
-          int p = 0, nb;
-          for (;; ++p) {
-            nb = va_tile_blocks<TREE>(q, P.tpt, p, 1);
-            if (cut[i] < u + (long long)nb * P.n_kv) break;
-            u += (long long)nb * P.n_kv;
-          }
-          int g = (int)((cut[i] - u) / nb), b = (int)((cut[i] - u) % nb);
-          long long at = cut[i];
-          if (nb <= VA_SNAP && b) {
-            if (2 * b < nb) {
-              at -= b;
+        if (cut[i] < e && cut[i] >= e - u) s_cut[i] = make_uint2(s0 + tid, cut[i] - (e - u));
+    }
+    __syncthreads();
+    // half of the threads look for each cut inside its sequence
+    const int i = tid / (VA_THREADS / 2), t = tid - i * (VA_THREADS / 2);
+    const int s = (int)s_cut[i].x;
+    if (s >= 0) {
+      const uint32_t u = s_cut[i].y;
+      const VaSeq q = va_seq<TREE>(P, s);
+      const int pairs = va_pairs(q, P.tpt), step = (pairs + VA_THREADS / 2 - 1) / (VA_THREADS / 2);
+      int p = t * step;
+      uint32_t at = p < pairs ? (va_blocks_before<TREE>(q, P.tpt, pairs, p) + p * VA_ITEM) * P.n_kv : 0u;
+      for (const int last = min(pairs, p + step); p < last; ++p) {
+        const uint32_t nb = va_tile_blocks<TREE>(q, P.tpt, p, 1), w = nb + VA_ITEM;
+        if (u >= at && u - at < w * P.n_kv) {   // one thread's
+          int g = (u - at) / w, b = (u - at) - g * w, np = p;
+          uint32_t place = cut[i];
+          if (b >= (int)nb || (nb <= VA_SNAP && b)) {
+            if (2 * b < (int)w) {
+              place -= b;
             } else {   // up to the next item
-              at += nb - b;
+              place += w - b;
               if (++g == P.n_kv) {
                 g = 0;
-                ++p;
+                ++np;
               }
             }
             b = 0;
           }
-          s_range[i] = at;
+          s_range[i] = place;
           if (i == 0) {
             int ns = s;
-            if (p == pairs) {   // (behind the sequence: the next one that has rows; unused at the list's end)
-              p = 0;
+            if (np == pairs) {   // (behind the sequence: the next one that has rows; unused at the list's end)
+              np = 0;
               do ++ns;
               while (ns < P.n_seqs && va_seq<TREE>(P, ns).n == 0);
             }
-            *s_at = {ns, p, g, b};
+            *s_at = {ns, np, g, b};
           }
         }
+        at += w * P.n_kv;
+      }
     }
   }
   tc_fence_before();
@@ -382,16 +531,18 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
   grid_dep_launch();   // this CTA holds its TMEM: dependents may start
 
   const int tpt = P.tpt, qpg = P.qpg;
-  if (warp >= 8) {
+  if (warp >= VA_WARP_TMA) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(VA_REGS_OTHER));
-  VaWalk<TREE> walk(P, start, units);
-  VaSegment seg;
-  if (warp == 8) {
+  VaWalk<TREE> seg(start, units);
+  if (warp == VA_WARP_TMA) {
     // ---- TMA: per segment K0, (Q), K1, V0, K2, V1, ..: the order the MMAs take them ----
     if (lane == 0) {
       int pos = 0, nseg = 0, q_loads = 0;
       bool ok = true;
-      for (; ok && walk.next(P, seg); ++nseg) {
+      int4 tail = make_int4(0, 0, 0, 0), first = make_int4(0, 0, 0, 0);   // this CTA's ends, for the joining kernel
+      for (; ok && seg.next(P); ++nseg) {
+        if (nseg == 0) first = make_int4(seg.b0 > 0, seg.b0 + seg.n == seg.nb, 0, 0);
+        if (seg.b0 == 0 && seg.n < seg.nb) tail = make_int4(seg.s, seg.p, seg.g, 1);
         auto load_q = [&] {
           if (nseg > 0) ok = mbar_wait_bounded(q_empty, (nseg - 1) & 1, P.err);
           if (!ok) return;
@@ -428,35 +579,37 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
       // every load has landed before the CTA may exit
       for (int i = max(0, pos - NS); i < pos; ++i) mbar_wait_bounded(&kv_full[i % NS], (i / NS) & 1, P.err);
       if (q_loads) mbar_wait_bounded(q_full, (q_loads - 1) & 1, P.err);
+      if (!ok) tail.w = first.x = 0;
+      P.head[2 * c] = tail;
+      P.head[2 * c + 1] = first;
     }
-  } else if (warp == 9) {
-    // ---- MMA issuer (lane 0; the warp's other lanes help to clear V rows) ----
+  } else if (warp == VA_WARP_MMA) {
+    // ---- MMA issuer (one lane; the others help to clear V rows) ----
     constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
     constexpr uint32_t ID_S = (1u << 4) | FMT | ((uint32_t)(VA_ROWS >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
     int ring = 0, nseg = 0, np[2] = {0, 0};
     bool ok = true;
-    for (; ok && walk.next(P, seg); ++nseg) {
+    for (; ok && seg.next(P); ++nseg) {
       const int n = seg.n, nbp = TREE ? va_blocks(seg.q.avail) : 0;
       auto at_k = [&](int i) { return ring + (i ? 2 * i - 1 : 0); };
       auto at_v = [&](int i) { return ring + (i < n - 1 ? 2 * i + 2 : 2 * n - 1); };
       auto wait = [&](uint64_t* bar, uint32_t ph) {
-        ok = __all_sync(0xffffffffu, ok && *abort_flag == 0 && mbar_wait_bounded(bar, ph, P.err));
+        ok = ok && va_wait(bar, ph, abort_flag, P.err);
         tc_fence_after();
       };
       auto kv_wait = [&](int at) { wait(&kv_full[at % NS], (at / NS) & 1); };
       auto kv_done = [&](int at) {
-        if (ok && lane == 0) mma_commit(&kv_empty[at % NS]);
+        if (ok && va_elect()) mma_commit(&kv_empty[at % NS]);
       };
-      auto mma_s = [&](int t, int i) {   // S_t = Q K(i)^T
-        kv_wait(at_k(i));
-        if (ok && lane == 0) {
-          const uint32_t qa = smem_u32(sm) + (seg.dual ? t : 0) * G::TILE;
-          const uint32_t ka = smem_u32(sm) + G::OFF_KV + (at_k(i) % NS) * G::TILE;
+      auto mma_s = [&](int t, int i) {   // S_t = Q K(i)^T (K(i) has been waited for)
+        const uint64_t qd = sdesc_sw128(smem_u32(sm) + (seg.dual ? t : 0) * G::TILE);
+        const uint64_t kd = sdesc_sw128(smem_u32(sm) + G::OFF_KV + (at_k(i) % NS) * G::TILE);
+        if (ok && va_elect()) {
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t o = (ks >> 2) * (VA_ROWS * 128) + (ks & 3) * 32;
-            mma_ss(tbase + G::S0 + t * 128, sdesc_sw128(qa + o), sdesc_sw128(ka + o), ID_S, ks > 0);
+            const uint32_t o = ((ks >> 2) * (VA_ROWS * 128) + (ks & 3) * 32) >> 4;
+            mma_ss(tbase + G::S0 + t * 128, qd + o, kd + o, ID_S, ks > 0);
           }
           mma_commit(&s_full[t]);
         }
@@ -475,22 +628,27 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
         }
       };
       auto mma_o = [&](int t, int i, bool first) {   // O_t += P_t V(i)
-        wait(&p_full[t], np[t]++ & 1);
-        if (ok && lane == 0) {
-          const uint32_t va = smem_u32(sm) + G::OFF_KV + (at_v(i) % NS) * G::TILE;
+        const uint64_t vd = sdesc_mn_sw128(smem_u32(sm) + G::OFF_KV + (at_v(i) % NS) * G::TILE, VA_ROWS * 128);
+        const uint32_t ph = np[t]++ & 1;
 #pragma unroll
-          for (int ks = 0; ks < VA_ROWS / 16; ++ks)
-            mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + ks * 8, sdesc_mn_sw128(va + ks * 2048, VA_ROWS * 128),
-                   ID_O, !(first && ks == 0));
+        for (int half = 0; half < 2; ++half) {
+          wait(&p_full[2 * t + half], ph);
+          if (ok && va_elect()) {
+#pragma unroll
+            for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+              mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + half * 64 + (ks & 3) * 8, vd + ks * (2048 >> 4), ID_O,
+                     !(first && ks == 0));
+          }
         }
       };
       auto o_done = [&](int t) {
-        if (ok && lane == 0) mma_commit(&o_full[t]);
+        if (ok && va_elect()) mma_commit(&o_full[t]);
       };
       auto q_done = [&] {
-        if (ok && lane == 0) mma_commit(q_empty);
+        if (ok && va_elect()) mma_commit(q_empty);
       };
       wait(q_full, nseg & 1);
+      kv_wait(at_k(0));
       if (seg.dual) {
         if (seg.n0 > 0) mma_s(0, 0);
         mma_s(1, 0);
@@ -498,6 +656,7 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
         if (n == 1) q_done();
         for (int i = 0; i < n && ok; ++i) {
           v_ready(i);
+          if (i + 1 < n) kv_wait(at_k(i + 1));
           if (i < seg.n0) {
             mma_o(0, i, i == 0);
             if (i + 1 < seg.n0) mma_s(0, i + 1);
@@ -515,12 +674,14 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
         }
       } else {
         for (int i = 0; i < 2 && i < n; ++i) {
+          kv_wait(at_k(i));
           mma_s(i, i);
           kv_done(at_k(i));
         }
         if (n <= 2) q_done();
         for (int i = 0; i < n && ok; ++i) {
           v_ready(i);
+          if (i + 2 < n) kv_wait(at_k(i + 2));
           mma_o(i & 1, i, i < 2);
           kv_done(at_v(i));
           if (i + 2 < n) {
@@ -536,37 +697,39 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
     }
     if (!ok) *abort_flag = 1;
     // every MMA issued here has retired before TMEM is released
-    if (lane == 0) {
-      mma_commit(done);
-      mbar_wait_bounded(done, 0, P.err);
-    }
+    __syncwarp();
+    if (va_elect()) mma_commit(done);
+    mbar_wait_bounded(done, 0, P.err);
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(VA_REGS_SOFTMAX));
-    VaWalk<TREE> walk(P, start, units);
-    VaSegment seg;
-    // ---- softmax group t: thread = row ----
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    VaWalk<TREE> seg(start, units);
+    // ---- softmax group t, half u: a thread has 64 of the 128 keys of a block for
+    //      one row, and half of the row's output columns.  Two warps make a pair
+    //      for 32 rows; every decision that a pair's barriers depend on is taken
+    //      by both (va_pair_any), so that none is left at one. ----
+    const int t = warp >> 3, u = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+    const int pair = t * 4 + (warp & 3), bar = 1 + pair;
     const uint32_t lanes = tbase + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_col = lanes + G::S0 + t * 128, o_col = lanes + G::O0 + t * HD;
+    const uint32_t s_col = lanes + G::S0 + t * 128 + u * 64, p_col = s_col;
+    const uint32_t o_col = lanes + G::O0 + t * HD + u * (HD / 2);
+    float* x_slot = s_x + t * VA_ROWS + row;
     const int tok_in_tile = row / qpg, head_in_group = row - tok_in_tile * qpg;
     const float scale = P.scale_log2;
     int ns = 0, nseg_o = 0, ng1 = 0;
     bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t ph) {
-      ok = __all_sync(0xffffffffu, ok && *abort_flag == 0 && mbar_wait_bounded(bar, ph, P.err));
+    auto wait = [&](uint64_t* b, uint32_t ph) {
+      ok = ok && va_wait(b, ph, abort_flag, P.err);
       tc_fence_after();
     };
-    int4 tail = make_int4(0, 0, 0, 0), first = make_int4(-1, 0, 0, 0);   // this CTA's ends, for the joining kernel
-    while (ok && walk.next(P, seg)) {
-      if (first.x < 0) first = make_int4(seg.b0 > 0, seg.b0 + seg.n == seg.nb, 0, 0);
-      if (seg.b0 == 0 && seg.n < seg.nb) tail = make_int4(seg.s, seg.p, seg.g, 1);
+    auto agree = [&] { ok = !va_pair_any(bar, !ok); };
+    while (ok && seg.next(P)) {
       const int tile = seg.dual ? t : 0;
       const int i_row = (2 * seg.p + tile) * tpt + tok_in_tile;      // query or node of this row
       const bool live = tok_in_tile < tpt && i_row < seg.q.n;
       const int nbp = TREE ? va_blocks(seg.q.avail) : 0;
       // packed: this row's keys, and the fewest any row of the tile sees
-      const int limit = TREE ? 0 : live ? va_limit(seg.q, i_row) : 0;
+      const int limit = TREE ? seg.q.avail : live ? va_limit(seg.q, i_row) : 0;
       const int tile_limit = TREE ? seg.q.avail : va_limit(seg.q, (2 * seg.p + tile) * tpt);
       const int step = seg.dual ? 1 : 2, n = seg.dual ? (t ? seg.n : seg.n0) : seg.n;
       float m = -INFINITY, l = 0.f;
@@ -574,46 +737,55 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
       for (int i = seg.dual ? 0 : t; i < n && ok; i += step) {
         const int b = seg.b0 + i, kb = b * VA_ROWS;
         const bool draft = TREE && b >= nbp;
-        uint4 bits = make_uint4(0u, 0u, 0u, 0u);
-        if (draft && live) {   // (before the wait: the load overlaps it)
-          const uint32_t* mrow = P.mask + ((size_t)seg.s * P.T + i_row) * P.words * 2;
-          const int w = (b - nbp) * 4;
-          const uint2 lo = *reinterpret_cast<const uint2*>(mrow + w);
-          const uint2 hi = w + 2 < 2 * P.words ? *reinterpret_cast<const uint2*>(mrow + w + 2) : make_uint2(0u, 0u);
-          const int valid = seg.q.n - (b - nbp) * VA_ROWS;
-          bits = make_uint4(lo.x & va_bits_below(valid, 0), lo.y & va_bits_below(valid, 1), hi.x & va_bits_below(valid, 2),
-                            hi.y & va_bits_below(valid, 3));
+        const bool masked = draft || kb + VA_ROWS > tile_limit;
+        uint2 bits = make_uint2(0u, 0u);
+        if (draft) {
+          const int word = (b - nbp) * 4 + u * 2, valid = seg.q.n - (b - nbp) * VA_ROWS;
+          if (live && word < 2 * P.words) {   // (before the wait: the load overlaps it)
+            bits = *reinterpret_cast<const uint2*>(P.mask + ((size_t)seg.s * P.T + i_row) * P.words * 2 + word);
+            bits = make_uint2(bits.x & va_bits_below(valid, 2 * u), bits.y & va_bits_below(valid, 2 * u + 1));
+          }
+        } else if (masked) {
+          bits = make_uint2(va_bits_below(limit - kb, 2 * u), va_bits_below(limit - kb, 2 * u + 1));
         }
         wait(&s_full[t], ns++ & 1);
-        if (!ok) break;
-        uint32_t s[128];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tmem_ld32(s_col + k * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[k * 32]));
-        tmem_ld_wait();
-        if (draft || kb + VA_ROWS > tile_limit) {
-          if (!draft) {
-            const int seen = (TREE ? seg.q.avail : limit) - kb;
-            bits = make_uint4(va_bits_below(seen, 0), va_bits_below(seen, 1), va_bits_below(seen, 2), va_bits_below(seen, 3));
-          }
-#pragma unroll
-          for (int e = 0; e < 128; ++e) {
-            const uint32_t w = e < 32 ? bits.x : e < 64 ? bits.y : e < 96 ? bits.z : bits.w;
-            if (!(w >> (e & 31) & 1u)) s[e] = 0xff800000u;   // -inf
-          }
-        }
         float mx[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = __uint_as_float(s[k]);
+        for (int k = 0; k < 2; ++k) {
+          uint32_t s[32];
+          tmem_ld32(s_col + k * 32, s);
+          tmem_ld_wait();
+          if (masked) {
 #pragma unroll
-        for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+            for (int e = 0; e < 32; ++e)
+              if (!((k == 0 ? bits.x : bits.y) >> e & 1u)) s[e] = 0xff800000u;   // -inf
+          }
+          if (k == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = __uint_as_float(s[e]);
+          }
+#pragma unroll
+          for (int e = k == 0 ? 4 : 0; e < 32; e += 2)
+            mx[(e >> 1) & 3] = va_max3(mx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+        }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-        if (__any_sync(0xffffffffu, top > m + VA_ROOM)) {
-          const float mn = fmaxf(m, top - VA_HEAD);
+        if (!ok) s_bad[pair] = 1;
+        // (behind this barrier both halves hold their scores: P may go over S)
+        if (va_pair_any(bar, top > m + VA_ROOM || !ok)) {
+          if (u) *x_slot = top;
+          va_pair_sync(bar);
+          if (s_bad[pair]) {
+            ok = false;
+            break;
+          }
+          if (!u) *x_slot = fmaxf(m, fmaxf(top, *x_slot) - VA_HEAD);
+          va_pair_sync(bar);
+          const float mn = *x_slot;
           if (any) {   // the rows of O so far follow the new reference
             const float f = mn == -INFINITY ? 1.f : va_ex2(m - mn);
             l *= f;
 #pragma unroll 1
-            for (int k = 0; k < HD / 32; ++k) {
+            for (int k = 0; k < HD / 64; ++k) {
               uint32_t o[32];
               tmem_ld32(o_col + k * 32, o);
               tmem_ld_wait();
@@ -621,47 +793,71 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tmem_st32(o_col + k * 32, o);
             }
+            tmem_st_wait();
           }
           m = mn;
+          tc_fence_before();
+          va_pair_sync(bar);   // both halves of O are ready before either half of P is announced
         }
         any = true;
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const f32x2 scale2 = va_pair(scale, scale), ref2 = va_pair(-ref, -ref);
+        f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t w[32];
+        for (int j = 0; j < 2; ++j) {
+          uint32_t w[16], s[32];
+          tmem_ld32(s_col + j * 32, s);
+          tmem_ld_wait();
+          if (masked) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float p0 = va_ex2(fmaf(__uint_as_float(s[k * 64 + 2 * e]), scale, -ref));
-            const float p1 = va_ex2(fmaf(__uint_as_float(s[k * 64 + 2 * e + 1]), scale, -ref));
-            sum[(2 * e) & 3] += p0;
-            sum[(2 * e + 1) & 3] += p1;
+            for (int e = 0; e < 32; ++e)
+              if (!((j == 0 ? bits.x : bits.y) >> e & 1u)) s[e] = 0xff800000u;   // -inf
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int i0 = 2 * e;
+            float p0, p1;
+            va_split(va_fma2(va_pair(__uint_as_float(s[i0]), __uint_as_float(s[i0 + 1])), scale2, ref2), p0, p1);
+            p0 = va_ex2(p0);
+            p1 = va_ex2(p1);
+            sum[e & 1] = va_add2(sum[e & 1], va_pair(p0, p1));
             w[e] = va_pack<F16>(p0, p1);
           }
-          tmem_st32(s_col + k * 32, w);
+          tmem_st16(p_col + j * 16, w);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full[2 * t + u]);
+        float l0, l1;
+        va_split(va_add2(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
       }
-      if (ok && any) wait(&o_full[t], nseg_o++ & 1);
       if (!ok) break;
+      if (any) wait(&o_full[t], nseg_o++ & 1);
+      agree();
+      if (!ok) break;
+      if (u) *x_slot = l;   // the row's sum
+      va_pair_sync(bar);
+      if (!u) *x_slot = l += *x_slot;
+      va_pair_sync(bar);
+      l = *x_slot;
       float f0 = 1.f, f1 = 0.f;
       const bool merge = !seg.dual && seg.n > 1;
       if (!seg.dual) {
         if (t == 1) {   // hand (m, l) and O_1 to group 0, and wait until it has read them
           if (!merge) continue;
-          s_ml[row] = make_float2(m, l);
+          if (!u) s_ml[row] = make_float2(m, l);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(g1_full);
           wait(g1_empty, ng1++ & 1);
+          agree();
           continue;
         }
         if (merge) {
-          wait(g1_full, ng1 & 1);
+          wait(g1_full, ng1++ & 1);
+          agree();
           if (!ok) break;
           const float2 other = s_ml[row];
           const float mn = fmaxf(m, other.x), ref = mn == -INFINITY ? 0.f : mn;
@@ -679,12 +875,31 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
         const float inv = l > 0.f ? 1.f / l : l;   // (a NaN stays one)
         f0 *= inv;
         f1 *= inv;
-        if (live && P.lse) P.lse[r * P.n_heads + h] = (m + __log2f(l)) * 0.6931471805599453f;
-      } else if (live) {
+        if (live && !u && P.lse) P.lse[r * P.n_heads + h] = (m + __log2f(l)) * 0.6931471805599453f;
+      } else if (live && !u) {
         P.part_ml[(size_t)slot * 256 + tile * VA_ROWS + row] = make_float2(m, l);
       }
+      // Rows leave in 16-byte pieces that a quad of lanes has transposed, so that
+      // a store covers 64 contiguous bytes of 8 rows and not 16 of 32.
+      uint8_t* start = nullptr;
+      if (live && any)
+        start = whole ? static_cast<uint8_t*>(P.out) + (r * P.o_row + h * P.o_head) * 2 + u * HD
+                     : reinterpret_cast<uint8_t*>(P.part_o + ((size_t)slot * 256 + tile * VA_ROWS + row) * HD + u * (HD / 2));
+      uint8_t* dst[4];   // this lane's piece of the quad's rows
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dst[j] = reinterpret_cast<uint8_t*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(start), (lane & ~3) + j));
+        if (dst[j]) dst[j] += (lane & 3) * 16;
+      }
+      auto store = [&](uint4 (&x)[4], int off) {
+        va_transpose(x, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (dst[j]) *reinterpret_cast<uint4*>(dst[j] + off) = x[j];
+      };
 #pragma unroll 1
-      for (int k = 0; k < HD / 32 && any; ++k) {
+      for (int k = 0; k < HD / 64 && any; ++k) {
         uint32_t o[32];
         tmem_ld32(o_col + k * 32, o);
         tmem_ld_wait();
@@ -699,92 +914,104 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f0);
         }
-        if (!live) continue;
+        uint4 x[4];
         if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(P.out) + r * P.o_row + h * P.o_head + k * 32);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float* f = reinterpret_cast<const float*>(&o[e * 8]);
-            dst[e] = make_uint4(va_pack_out(f[0], f[1], P.out_f16), va_pack_out(f[2], f[3], P.out_f16),
-                                va_pack_out(f[4], f[5], P.out_f16), va_pack_out(f[6], f[7], P.out_f16));
+            x[e] = make_uint4(va_pack_out(f[0], f[1], P.out_f16), va_pack_out(f[2], f[3], P.out_f16),
+                              va_pack_out(f[4], f[5], P.out_f16), va_pack_out(f[6], f[7], P.out_f16));
           }
+          store(x, k * 64);
         } else {
-          uint4* dst = reinterpret_cast<uint4*>(P.part_o + ((size_t)slot * 256 + tile * VA_ROWS + row) * HD + k * 32);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = half * 16 + e * 4;
+              x[e] = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+            store(x, k * 128 + half * 64);
+          }
         }
       }
       tc_fence_before();
       if (merge) {
-        ++ng1;
         __syncwarp();
         if (lane == 0) mbar_arrive(g1_empty);
       }
     }
     if (!ok) *abort_flag = 1;
-    if (tid == 0) {
-      P.head[2 * c] = tail;
-      P.head[2 * c + 1] = make_int4(ok && first.x > 0, first.y, 0, 0);
-    }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == VA_WARP_MMA) {
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
 }
 
-// Joins the partials of the items that were cut: block (c, y) takes rows 32 y
-// .. 32 y + 31 of the item that begins in CTA c and ends in a later one.  The
-// pieces are CTA c's last and the first of the CTAs after it, in that order.
+// Joins the partials of the items that were cut: block (c, y) takes a few rows
+// of the item that begins in CTA c and ends in a later one.  The pieces are
+// CTA c's last and the first of the CTAs after it, joined in that order.  The
+// loads of eight pieces are in flight at once.
 template <int HD, bool TREE>
 __global__ void __launch_bounds__(256) varlen_join_kernel(const __grid_constant__ VaParams P, int grid) {
+  constexpr int LPR = HD / 4, ROWS = 256 / LPR, BATCH = 8;   // threads per row, rows per block
   grid_dep_wait();
   grid_dep_launch();
   const int c = blockIdx.x;
   const int4 tail = P.head[2 * c];
   if (!tail.w) return;
+  const VaSeq q = va_seq<TREE>(P, tail.x);
+  const int row = blockIdx.y * ROWS + threadIdx.x / LPR, col = (threadIdx.x % LPR) * 4;
+  const int tile = row / VA_ROWS, in_tile = row % VA_ROWS;
+  const int tok = in_tile / P.qpg, i_row = (2 * tail.y + tile) * P.tpt + tok;
+  if (tok >= P.tpt || i_row >= q.n) return;
   int last = c;
   for (;;) {
-    ++last;
-    if (last >= grid) return;   // (a CTA gave up: its word says so)
+    if (++last >= grid) return;   // (a CTA gave up: the status word says so)
     const int4 f = P.head[2 * last + 1];
     if (!f.x) return;
     if (f.y) break;
   }
-  const VaSeq q = va_seq<TREE>(P, tail.x);
-  constexpr int LPR = HD / 4, RPB = 256 / LPR;   // threads per row, rows at once
-  const int col = (threadIdx.x % LPR) * 4;
-  for (int rr = threadIdx.x / LPR; rr < 32; rr += RPB) {
-    const int row = blockIdx.y * 32 + rr, tile = row / VA_ROWS, in_tile = row % VA_ROWS;
-    const int tok = in_tile / P.qpg, i_row = (2 * tail.y + tile) * P.tpt + tok;
-    if (tok >= P.tpt || i_row >= q.n) continue;
-    const size_t at0 = (size_t)(2 * c + 1) * 256 + row;
-    float m = P.part_ml[at0].x;
-    for (int j = c + 1; j <= last; ++j) m = fmaxf(m, P.part_ml[(size_t)(2 * j) * 256 + row].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = c; j <= last; ++j) {
-      const size_t at = j == c ? at0 : (size_t)(2 * j) * 256 + row;
-      const float2 ml = P.part_ml[at];
-      if (ml.x == -INFINITY) continue;   // no key of this row in the piece (its O may not be written)
-      const float f = va_ex2(ml.x - ref);
-      const float4 x = *reinterpret_cast<const float4*>(P.part_o + at * HD + col);
-      l += ml.y * f;
-      o.x += x.x * f;
-      o.y += x.y * f;
-      o.z += x.z * f;
-      o.w += x.w * f;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = c; j0 <= last; j0 += BATCH) {
+    float2 ml[BATCH];
+    float4 x[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int j = j0 + k;
+      const size_t at = (size_t)(2 * j + (j == c)) * 256 + row;
+      ml[k] = j <= last ? P.part_ml[at] : make_float2(-INFINITY, 0.f);
+      x[k] = j <= last ? *reinterpret_cast<const float4*>(P.part_o + at * HD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const float inv = l > 0.f ? 1.f / l : l;
-    const int h = tail.z * P.qpg + in_tile - tok * P.qpg;
-    const size_t r = (size_t)(q.q0 + i_row);
-    uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + r * P.o_row + h * P.o_head + col);
-    *dst = make_uint2(va_pack_out(o.x * inv, o.y * inv, P.out_f16), va_pack_out(o.z * inv, o.w * inv, P.out_f16));
-    if (P.lse && col == 0) P.lse[r * P.n_heads + h] = (m + __log2f(l)) * 0.6931471805599453f;
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) mn = fmaxf(mn, ml[k].x);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float f = va_ex2(m - ref);
+    l *= f;
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      if (ml[k].x == -INFINITY) continue;   // no key of this row in the piece (its O may not be written)
+      const float w = va_ex2(ml[k].x - ref);
+      l += ml[k].y * w;
+      o.x += x[k].x * w;
+      o.y += x[k].y * w;
+      o.z += x[k].z * w;
+      o.w += x[k].w * w;
+    }
+    m = mn;
   }
+  const float inv = l > 0.f ? 1.f / l : l;
+  const int h = tail.z * P.qpg + in_tile - tok * P.qpg;
+  const size_t r = (size_t)(q.q0 + i_row);
+  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + r * P.o_row + h * P.o_head + col);
+  *dst = make_uint2(va_pack_out(o.x * inv, o.y * inv, P.out_f16), va_pack_out(o.z * inv, o.w * inv, P.out_f16));
+  if (P.lse && col == 0) P.lse[r * P.n_heads + h] = (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------
@@ -830,7 +1057,7 @@ static int va_launch_t(VaParams& P, int grid, bool join, cudaStream_t st) {
   if (allow_smem(kern, VaGeom<HD>::BYTES) != T2B_OK) return T2B_ERR_LAUNCH;
   const int rc = launch_pdl(kern, dim3(grid), dim3(VA_THREADS), (size_t)VaGeom<HD>::BYTES, st, P);
   if (rc != T2B_OK || !join) return rc;
-  return launch_pdl(varlen_join_kernel<HD, TREE>, dim3(grid, 8), dim3(256), 0, st, P, grid);
+  return launch_pdl(varlen_join_kernel<HD, TREE>, dim3(grid, 256 * (HD / 4) / 256), dim3(256), 0, st, P, grid);
 }
 
 // max_blocks: no item has more blocks of keys; pairs: no more (sequence, pair of tiles).
@@ -848,7 +1075,8 @@ static int va_launch(VaParams& P, int hd, bool f16, const void* q, size_t q_row,
   int dev = 0, sms = VA_MAX_CTAS;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return T2B_ERR_LAUNCH;
-  const long long units = pairs * max_blocks * P.n_kv;
+  const long long units = pairs * (max_blocks + VA_ITEM) * P.n_kv;
+  if (units > 0x7fffffffll) return T2B_ERR_SHAPE;
   const int grid = (int)std::max(1ll, std::min<long long>({units / VA_MIN_UNITS, sms, VA_MAX_CTAS}));
   const bool join = grid > 1 && max_blocks > VA_SNAP;
   const bool tree = P.T > 0;
