@@ -16,11 +16,12 @@
 //
 // Alternatives: a value and its index form one 64-bit key (order-preserving
 // value bits << 32 | ~index: larger value first, ties to the lower index).
-// Candidates above the K-th best key so far are appended to a shared list
-// that is cut back to K when it fills.  The bound for the first chunk (and
-// for a chunk that would overflow the list) is the K-th largest of 64 group
-// maxima: at least K keys reach it, and at most K groups of 128 values hold
-// one, so the list cannot overflow whatever the order of the logits.
+// A thread whose chunk maximum passes the K-th best value so far appends its
+// candidates to a shared list, which is cut back to K when it has grown.  The
+// first chunk is bounded by the K-th largest of 64 group maxima instead: at
+// least K values reach it.  Where ties or an unlucky order would overflow the
+// list, the chunk is bounded by whole keys: those are distinct, so at most K
+// groups of 128 values hold a candidate and the list suffices for any order.
 
 #include <math.h>
 
@@ -73,6 +74,12 @@ T2B_DEV u64 lp_quad_max(u64 k) {
   return k;
 }
 
+T2B_DEV float lp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Running (m, s, z) of a set of values; z is relative to m.
 struct LpSum {
   float m, s, z;
@@ -80,7 +87,7 @@ struct LpSum {
 T2B_DEV LpSum lp_rescale(LpSum a, float m) {
   if (a.m == m || a.m == -INFINITY) return {m, a.s, a.z};   // nothing but -inf so far: s = z = 0
   const float d = fmaxf(a.m - m, -1e30f);                     // (a difference that overflows has c = 0)
-  const float c = exp2f(d * LP_LOG2E);
+  const float c = lp_ex2(d * LP_LOG2E);
   return {m, a.s * c, (a.z + a.s * d) * c};
 }
 T2B_DEV LpSum lp_join(LpSum a, LpSum b) {
@@ -104,6 +111,7 @@ struct LpShared {
   u64 top[LP_MAX_TOP];
   u64 group[LP_GROUPS];
   u64 bound;
+  float value_bound;
   LpSum sum[LP_THREADS / 32];
   int n;
 };
@@ -124,6 +132,30 @@ T2B_DEV void lp_group_bound(LpShared& S, u64 mine, int K) {
     if (rank == K - 1 && k) S.bound = k;   // keys are distinct: one group at most
   }
   __syncthreads();
+}
+
+// The same on values: at least K values of the chunk reach it (-inf where
+// fewer than K groups have one).
+T2B_DEV float lp_group_value(LpShared& S, float mine, int K) {
+  const int tid = threadIdx.x;
+  float* group = reinterpret_cast<float*>(S.group);
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+  if ((tid & 3) == 0) group[tid >> 2] = mine;
+  if (tid == 0) S.value_bound = -INFINITY;
+  __syncthreads();
+  if (tid < LP_GROUPS) {
+    const float v = group[tid];
+    int above = 0, from = 0;
+#pragma unroll 16
+    for (int i = 0; i < LP_GROUPS; ++i) {
+      above += group[i] > v;
+      from += group[i] >= v;
+    }
+    if (above < K && from >= K) S.value_bound = v;   // (every thread that writes holds the same value)
+  }
+  __syncthreads();
+  return S.value_bound;
 }
 
 // Cut the list of S.n keys to its K largest, in order, at list[0..K); empty
@@ -154,6 +186,7 @@ T2B_DEV void lp_cut(LpShared& S, int K) {
   for (int i = tid; i < n; i += LP_THREADS) {
     const u64 k = S.list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += S.list[j] > k;
     if (rank < K && k) S.top[rank] = k;
   }
@@ -176,7 +209,7 @@ T2B_DEV float lp_peer_f32(const float* p, uint32_t rank) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const LpParams P) {
+__global__ void __launch_bounds__(LP_THREADS, 3) token_logprobs_kernel(const LpParams P) {
   constexpr int VEC = 16 / sizeof(T), NV = LP_PER / VEC;
   __shared__ LpShared S;
   grid_dep_wait();
@@ -191,79 +224,121 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const LpPara
   const int shift = (int)((reinterpret_cast<uintptr_t>(x + v0) % 16) / sizeof(T));
   const int base = v0 - shift;
   LpSum a = {-INFINITY, 0.f, 0.f};
+  float floor = -INFINITY;   // the K-th best value at the last cut: only larger ones are candidates
   if (tid == 0) S.n = 0;
   __syncthreads();
-  bool first = true;
   for (int c0 = base; c0 < v1; c0 += LP_CHUNK) {
     float v[LP_PER];
+    if (c0 >= v0 && c0 + LP_CHUNK <= v1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int g = c0 + (i * LP_THREADS + tid) * VEC;
-      if (g >= v0 && g + VEC <= v1) {
-        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + g));
+      for (int i = 0; i < NV; ++i) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + c0 + (i * LP_THREADS + tid) * VEC));
         const T* t = reinterpret_cast<const T*>(&w);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[i * VEC + e] = lp_float<T>(t[e]);
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i * VEC + e] = g + e >= v0 && g + e < v1 ? lp_float<T>(x[g + e]) : -INFINITY;
+      for (int i = 0; i < NV; ++i) {
+        const int g = c0 + (i * LP_THREADS + tid) * VEC;
+        if (g >= v0 && g + VEC <= v1) {
+          const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + g));
+          const T* t = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[i * VEC + e] = lp_float<T>(t[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[i * VEC + e] = g + e >= v0 && g + e < v1 ? lp_float<T>(x[g + e]) : -INFINITY;
+        }
       }
     }
-    float cm = v[0];
+    float hi[2] = {v[0], v[1]}, lo[2] = {v[0], v[1]};
 #pragma unroll
-    for (int e = 1; e < LP_PER; ++e) cm = fmaxf(cm, v[e]);
+    for (int e = 2; e < LP_PER; ++e) {
+      hi[e & 1] = fmaxf(hi[e & 1], v[e]);
+      lo[e & 1] = fminf(lo[e & 1], v[e]);
+    }
+    const float cm = fmaxf(hi[0], hi[1]);
     if (cm > a.m) a = lp_rescale(a, cm);
     const float ms = a.m == -INFINITY ? 0.f : a.m;
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, z[4] = {0.f, 0.f, 0.f, 0.f};
+    if (fminf(lo[0], lo[1]) > -1e30f) {
 #pragma unroll
-    for (int e = 0; e < LP_PER; ++e) {
-      const float d = v[e] - ms, p = exp2f(d * LP_LOG2E);
-      a.s += p;
-      a.z += p * fmaxf(d, -1e30f);   // a masked value (-inf) adds nothing
+      for (int e = 0; e < LP_PER; ++e) {
+        const float d = v[e] - ms, p = lp_ex2(d * LP_LOG2E);
+        s[e & 3] += p;
+        z[e & 3] = fmaf(p, d, z[e & 3]);
+      }
+    } else {   // masked values (-inf) add nothing
+#pragma unroll
+      for (int e = 0; e < LP_PER; ++e) {
+        const float d = v[e] - ms, p = lp_ex2(d * LP_LOG2E);
+        s[e & 3] += p;
+        z[e & 3] = fmaf(p, fmaxf(d, -1e30f), z[e & 3]);
+      }
     }
+    a.s += (s[0] + s[1]) + (s[2] + s[3]);
+    a.z += (z[0] + z[1]) + (z[2] + z[3]);
     if (K) {
       auto index = [&](int e) { return c0 + ((e / VEC) * LP_THREADS + tid) * VEC + e % VEC; };
       auto inside = [&](int e) { return index(e) >= v0 && index(e) < v1; };
-      bool bounded = first;
-      const int before = S.n;   // (a barrier lies between this and the last append)
-      if (!first) {
-        // values tied with the K-th best so far have a higher index and lose
-        const float floor = before >= K ? lp_value(S.list[K - 1]) : NAN;
-        __syncthreads();
+      const bool first = c0 == base;
+      if (first) floor = lp_group_value(S, cm, K);
+      int at = 0;
+      // (later values tied with the K-th best so far have a higher index and lose)
+      if (first ? !(cm < floor) : cm > floor) {
+        uint32_t hits = 0;
 #pragma unroll
-        for (int e = 0; e < LP_PER; ++e)
-          if (!(v[e] <= floor) && inside(e)) {
-            const int at = atomicAdd(&S.n, 1);
-            if (at < LP_CAP) S.list[at] = lp_key(v[e], index(e));
-          }
-        __syncthreads();
-        if (S.n > LP_CAP) {   // drop this chunk's, bound it, append again
-          __syncthreads();
-          if (tid == 0) S.n = before;
-          __syncthreads();
-          lp_cut(S, K);
-          bounded = true;
+        for (int e = 0; e < LP_PER; ++e) hits |= (uint32_t)(first ? !(v[e] < floor) : v[e] > floor) << e;
+        while (hits) {   // a lane has one candidate or two; taking its value by selects keeps v in registers
+          const int h = __ffs(hits) - 1;
+          hits &= hits - 1;
+          float value = v[0];
+#pragma unroll
+          for (int e = 1; e < LP_PER; ++e) value = e == h ? v[e] : value;
+          if (!inside(h)) continue;
+          at = atomicAdd(&S.n, 1);
+          if (at < LP_CAP) S.list[at] = lp_key(value, index(h));
         }
       }
-      if (bounded) {
-        u64 mine = 0;
+      if (__syncthreads_or(first || at >= LP_CUT)) {
+        if (S.n > LP_CAP) {   // this chunk's candidates again, bounded by whole keys
+          const int n = LP_CAP;
+          constexpr int R = (LP_CAP + LP_THREADS - 1) / LP_THREADS;
+          u64 keep[R];
 #pragma unroll
-        for (int e = 0; e < LP_PER; ++e)
-          if (inside(e)) {
-            const u64 k = lp_key(v[e], index(e));
-            mine = k > mine ? k : mine;
+          for (int r = 0; r < R; ++r) {
+            const u64 k = tid + r * LP_THREADS < n ? S.list[tid + r * LP_THREADS] : 0;
+            keep[r] = (int)(0xFFFFFFFFu - (uint32_t)k) < c0 ? k : 0;   // of earlier chunks
           }
-        lp_group_bound(S, mine, K);
-        const u64 bound = S.bound;
+          __syncthreads();
+          if (tid == 0) S.n = 0;
+          __syncthreads();
 #pragma unroll
-        for (int e = 0; e < LP_PER; ++e)
-          if (inside(e)) {
-            const u64 k = lp_key(v[e], index(e));
-            if (k >= bound) S.list[atomicAdd(&S.n, 1)] = k;
-          }
-        __syncthreads();
+          for (int r = 0; r < R; ++r)
+            if (keep[r]) S.list[atomicAdd(&S.n, 1)] = keep[r];
+          __syncthreads();
+          lp_cut(S, K);
+          u64 mine = 0;
+#pragma unroll
+          for (int e = 0; e < LP_PER; ++e)
+            if (inside(e)) {
+              const u64 k = lp_key(v[e], index(e));
+              mine = k > mine ? k : mine;
+            }
+          lp_group_bound(S, mine, K);
+          const u64 bound = S.bound;
+#pragma unroll
+          for (int e = 0; e < LP_PER; ++e)
+            if (inside(e)) {
+              const u64 k = lp_key(v[e], index(e));
+              if (k >= bound) S.list[atomicAdd(&S.n, 1)] = k;
+            }
+          __syncthreads();
+        }
+        lp_cut(S, K);
+        floor = S.n < K ? -INFINITY : lp_value(S.list[K - 1]);
       }
-      first = false;
-      if (S.n > LP_CUT || bounded) lp_cut(S, K);
     }
   }
   // ---- the CTA's sums, in a fixed order ----
