@@ -139,6 +139,11 @@ def stream(s: torch.cuda.Stream | None = None) -> int:
     return (s or torch.cuda.current_stream()).cuda_stream
 
 
+def raw_stream(dev: int) -> int:
+    """Handle of the current stream of device ``dev``, without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 @contextmanager
 def status_word(word: torch.Tensor, st: int):
     """Launches on stream ``st`` inside this block record timed-out device waits

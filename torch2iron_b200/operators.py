@@ -416,30 +416,43 @@ class CopyPresentPacketKV:
 # ---------------------------------------------------------------------------
 # serving operators
 # ---------------------------------------------------------------------------
-def _check_arg(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, contiguous: bool = True) -> None:
-    """Shape, type, device and layout of one argument (``shape`` entries of None match anything)."""
-    if tuple(t.shape) != shape and (t.dim() != len(shape) or
-                                    any(want is not None and n != want for n, want in zip(t.shape, shape))):
-        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+def _check_arg(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, dev: int, contiguous: bool = True) -> None:
+    """Shape, type, device (the current one, ``dev``) and layout of one argument."""
+    if t.shape == shape and t.dtype is dtype and t.get_device() == dev and (not contiguous or t.is_contiguous()):
+        return
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if not t.is_cuda or t.get_device() != dev:
         raise ValueError(f"{name}: expected a tensor on the current CUDA device, got {t.device}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous")
+    raise ValueError(f"{name}: must be contiguous")
+
+
+def _current_device(t: torch.Tensor) -> int:
+    """The current device's index (-2, which no tensor has, where there is none)."""
+    return torch.cuda.current_device() if t.is_cuda else -2
 
 
 def _strides(name: str, t: torch.Tensor) -> list[int]:
     """Element strides of every axis but the last (contiguous) one, as the
     kernels take them: nonzero multiples of 8 on a 16-byte aligned base."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape, strides = t.shape, t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: the last axis must be contiguous")
     if t.data_ptr() % 16:
         raise ValueError(f"{name}: must start on a 16-byte boundary")
-    out = [s if n > 1 else 8 for n, s in zip(t.shape[:-1], t.stride())]    # an axis of one has no stride
-    if any(s % 8 or s <= 0 for s in out):
-        raise ValueError(f"{name}: strides {tuple(t.stride())} must be nonzero multiples of 8 elements")
+    out = []
+    for i in range(len(shape) - 1):
+        s = strides[i] if shape[i] > 1 else 8          # an axis of one has no stride
+        if s % 8 or s <= 0:
+            raise ValueError(f"{name}: strides {strides} must be nonzero multiples of 8 elements")
+        out.append(s)
     return out
+
+
+def _addr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _check_heads(op) -> None:
@@ -515,35 +528,40 @@ class PackedAttention:
                 ArgSpec("out", q, self.out_dtype)]
 
     def __call__(self, q, k, v, q_start, out, k_start=None, k_len=None, lse=None):
-        for t, spec, nm in zip((q, k, v, q_start, out), self.get_arg_spec(), ("q", "k", "v", "q_start", "out")):
-            _check_arg(nm, t, spec.shape, spec.dtype, contiguous=t is q_start)
-        cached = self.max_ctx is not None
+        dev, cached, i32 = _current_device(q), self.max_ctx is not None, torch.int32
+        rows, kv = (self.tokens, self.num_heads, self.head_dim), self._kv_shape()
+        _check_arg("q", q, rows, self.dtype, dev, False)
+        _check_arg("k", k, kv, self.dtype, dev, False)
+        _check_arg("v", v, kv, self.dtype, dev, False)
+        _check_arg("q_start", q_start, (self.num_seqs + 1,), i32, dev)
+        _check_arg("out", out, rows, self.out_dtype, dev, False)
         if cached and (k_start is not None or k_len is None):
             raise ValueError("cache rows take k_len and no k_start")
         if not cached and (k_start is None) != (k_len is None):
             raise ValueError("packed keys take k_start and k_len together")
         if not cached and k_start is None and self.kv_tokens != self.tokens:
             raise ValueError("keys without k_start are packed as the queries are: kv_tokens must equal tokens")
-        for nm, t in (("k_start", k_start), ("k_len", k_len)):
-            if t is not None:
-                _check_arg(nm, t, (self.num_seqs,), torch.int32)
+        if k_start is not None:
+            _check_arg("k_start", k_start, (self.num_seqs,), i32, dev)
+        if k_len is not None:
+            _check_arg("k_len", k_len, (self.num_seqs,), i32, dev)
         if lse is not None:
-            _check_arg("lse", lse, (self.tokens, self.num_heads), torch.float32)
-        qs, os = _strides("q", q), _strides("out", out)
-        ks, vs = _strides("k", k), _strides("v", v)
+            _check_arg("lse", lse, rows[:2], torch.float32, dev)
+        qs, os, ks, vs = _strides("q", q), _strides("out", out), _strides("k", k), _strides("v", v)
         if cached:       # (row, head, token) -> (token, head, row)
-            ks, vs = ks[::-1], vs[::-1]
+            ks.reverse()
+            vs.reverse()
         else:
-            ks, vs = ks + [8], vs + [8]
-        L = _lib.lib()
+            ks.append(8)
+            vs.append(8)
+        L = _lib.load()
         n = L.t2b_varlen_attention_workspace_bytes(self.head_dim)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        p = _lib.ptr
         _lib.check("t2b_packed_attention", L.t2b_packed_attention(
-            p(q), p(k), p(v), p(out), p(lse), _lib.DTYPE[self.dtype], _lib.DTYPE[self.out_dtype], p(q_start),
-            p(k_start), p(k_len), self.num_seqs, self.tokens, self.num_seqs if cached else 0,
-            self.max_ctx if cached else self.kv_tokens, self.num_heads, self.num_kv_groups, self.head_dim, *qs, *os,
-            *ks, *vs, self.scale, p(ws), n, _lib.stream()))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _addr(lse), _lib.DTYPE[self.dtype],
+            _lib.DTYPE[self.out_dtype], q_start.data_ptr(), _addr(k_start), _addr(k_len), self.num_seqs, self.tokens,
+            self.num_seqs if cached else 0, kv[2] if cached else kv[0], rows[1], self.num_kv_groups, self.head_dim, *qs,
+            *os, *ks, *vs, self.scale, ws.data_ptr(), n, _lib.raw_stream(dev)))
         return out
 
 
@@ -632,24 +650,33 @@ class DraftTreeAttention:
                 ArgSpec("in", (self.batch, self.nodes, self.mask_words), torch.int64), ArgSpec("out", q, self.out_dtype)]
 
     def __call__(self, q, k_cache, v_cache, k_draft, v_draft, ctx_len, mask, out, num_nodes=None, lse=None):
-        names = ("q", "k_cache", "v_cache", "k_draft", "v_draft", "ctx_len", "mask", "out")
-        for t, spec, nm in zip((q, k_cache, v_cache, k_draft, v_draft, ctx_len, mask, out), self.get_arg_spec(), names):
-            _check_arg(nm, t, spec.shape, spec.dtype, contiguous=nm in ("k_cache", "v_cache", "ctx_len", "mask"))
+        dev, B, T, hd = _current_device(q), self.batch, self.nodes, self.head_dim
+        rows, draft = (B, T, self.num_heads, hd), (B, T, self.num_kv_groups, hd)
+        cache = (B, self.num_kv_groups, self.max_ctx, hd)
+        _check_arg("q", q, rows, self.dtype, dev, False)
+        _check_arg("k_cache", k_cache, cache, self.dtype, dev)
+        _check_arg("v_cache", v_cache, cache, self.dtype, dev)
+        _check_arg("k_draft", k_draft, draft, self.dtype, dev, False)
+        _check_arg("v_draft", v_draft, draft, self.dtype, dev, False)
+        _check_arg("ctx_len", ctx_len, (B,), torch.int32, dev)
+        _check_arg("mask", mask, (B, T, self.mask_words), torch.int64, dev)
+        _check_arg("out", out, rows, self.out_dtype, dev, False)
         if num_nodes is not None:
-            _check_arg("num_nodes", num_nodes, (self.batch,), torch.int32)
+            _check_arg("num_nodes", num_nodes, (B,), torch.int32, dev)
         if lse is not None:
-            _check_arg("lse", lse, (self.batch, self.nodes, self.num_heads), torch.float32)
+            _check_arg("lse", lse, rows[:3], torch.float32, dev)
+        if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+            raise ValueError("the caches must start on a 16-byte boundary")
         qs, os = self._rows("q", q), self._rows("out", out)
         kd, vd = _strides("k_draft", k_draft), _strides("v_draft", v_draft)
-        _strides("k_cache", k_cache), _strides("v_cache", v_cache)
-        L = _lib.lib()
-        n = L.t2b_varlen_attention_workspace_bytes(self.head_dim)
+        L = _lib.load()
+        n = L.t2b_varlen_attention_workspace_bytes(hd)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        p = _lib.ptr
         _lib.check("t2b_tree_attention", L.t2b_tree_attention(
-            p(q), p(k_cache), p(v_cache), p(k_draft), p(v_draft), p(out), p(lse), _lib.DTYPE[self.dtype],
-            _lib.DTYPE[self.out_dtype], p(ctx_len), p(num_nodes), p(mask), self.batch, self.nodes, self.num_heads,
-            self.num_kv_groups, self.head_dim, self.max_ctx, *qs, *os, *kd, *vd, self.scale, p(ws), n, _lib.stream()))
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_draft.data_ptr(), v_draft.data_ptr(), out.data_ptr(),
+            _addr(lse), _lib.DTYPE[self.dtype], _lib.DTYPE[self.out_dtype], ctx_len.data_ptr(), _addr(num_nodes),
+            mask.data_ptr(), B, T, rows[2], self.num_kv_groups, hd, self.max_ctx, *qs, *os, *kd, *vd, self.scale,
+            ws.data_ptr(), n, _lib.raw_stream(dev)))
         return out
 
     def _rows(self, name, t) -> list[int]:
@@ -708,47 +735,52 @@ class DraftTreeCommit:
                 ArgSpec("out", (self.batch,), i32), ArgSpec("out", (self.batch,), i32),
                 ArgSpec("out", (self.batch,), i32)]
 
-    def _layers(self, name: str, ts, shape: tuple, contiguous: bool):
+    def _layers(self, name: str, ts, shape: tuple, dev: int, contiguous: bool):
         """Host array of the layers' device pointers, and the strides they share."""
         if isinstance(ts, torch.Tensor):
-            _check_arg(name, ts, (self.layers, *shape), self.dtype, contiguous=False)
-            one, step = ts[0], ts.stride(0) * ts.element_size()
-            at = [ts.data_ptr() + i * step for i in range(self.layers)]
+            _check_arg(name, ts, (self.layers, *shape), self.dtype, dev, False)
+            strides = _strides(name, ts)
+            step, base = strides[0] * ts.element_size(), ts.data_ptr()
+            at, strides = range(base, base + step * self.layers, step), strides[1:]
+            if contiguous and not ts[0].is_contiguous():
+                raise ValueError(f"{name}: must be contiguous")
         else:
             if len(ts) != self.layers:
                 raise ValueError(f"{name}: expected {self.layers} layers, got {len(ts)}")
-            one = ts[0]
+            layout = ts[0].stride()
             for t in ts:
-                _check_arg(name, t, shape, self.dtype, contiguous=False)
-                if t.stride() != one.stride():
+                _check_arg(name, t, shape, self.dtype, dev, contiguous)
+                if t.stride() != layout:
                     raise ValueError(f"{name}: the layers' strides differ")
+            strides = _strides(name, ts[0])
             at = [t.data_ptr() for t in ts]
-        if contiguous and not one.is_contiguous():
-            raise ValueError(f"{name}: must be contiguous")
-        strides = _strides(name, one)
-        if any(a % 16 for a in at):
-            raise ValueError(f"{name}: must start on a 16-byte boundary")
+            if any(a % 16 for a in at):
+                raise ValueError(f"{name}: must start on a 16-byte boundary")
         return (ctypes.c_void_p * self.layers)(*at), strides
 
     def __call__(self, tokens, parents, predicted, ctx_len, k_drafts, v_drafts, k_caches, v_caches, path, num_accepted,
                  next_token, new_len, num_nodes=None):
-        i32, tree, row = torch.int32, (self.batch, self.nodes), (self.batch,)
-        for nm, t, shape in (("tokens", tokens, tree), ("parents", parents, tree), ("predicted", predicted, tree),
-                             ("ctx_len", ctx_len, row), ("path", path, tree), ("num_accepted", num_accepted, row),
-                             ("next_token", next_token, row), ("new_len", new_len, row)):
-            _check_arg(nm, t, shape, i32)
+        dev, i32, tree, row = _current_device(tokens), torch.int32, (self.batch, self.nodes), (self.batch,)
+        _check_arg("tokens", tokens, tree, i32, dev)
+        _check_arg("parents", parents, tree, i32, dev)
+        _check_arg("predicted", predicted, tree, i32, dev)
+        _check_arg("ctx_len", ctx_len, row, i32, dev)
+        _check_arg("path", path, tree, i32, dev)
+        _check_arg("num_accepted", num_accepted, row, i32, dev)
+        _check_arg("next_token", next_token, row, i32, dev)
+        _check_arg("new_len", new_len, row, i32, dev)
         if num_nodes is not None:
-            _check_arg("num_nodes", num_nodes, row, i32)
+            _check_arg("num_nodes", num_nodes, row, i32, dev)
         draft = (self.batch, self.nodes, self.num_kv_groups, self.head_dim)
         cache = (self.batch, self.num_kv_groups, self.max_ctx, self.head_dim)
-        kd, kds = self._layers("k_drafts", k_drafts, draft, False)
-        vd, vds = self._layers("v_drafts", v_drafts, draft, False)
-        kc, _ = self._layers("k_caches", k_caches, cache, True)
-        vc, _ = self._layers("v_caches", v_caches, cache, True)
-        p = _lib.ptr
-        _lib.call("t2b_tree_commit", p(tokens), p(parents), p(predicted), p(ctx_len), p(num_nodes), kd, vd, kc, vc,
-                  self.layers, p(path), p(num_accepted), p(next_token), p(new_len), self.batch, self.nodes,
-                  self.num_kv_groups, self.head_dim, self.max_ctx, *kds, *vds, _lib.stream())
+        kd, kds = self._layers("k_drafts", k_drafts, draft, dev, False)
+        vd, vds = self._layers("v_drafts", v_drafts, draft, dev, False)
+        kc, _ = self._layers("k_caches", k_caches, cache, dev, True)
+        vc, _ = self._layers("v_caches", v_caches, cache, dev, True)
+        _lib.check("t2b_tree_commit", _lib.load().t2b_tree_commit(
+            tokens.data_ptr(), parents.data_ptr(), predicted.data_ptr(), ctx_len.data_ptr(), _addr(num_nodes), kd, vd, kc,
+            vc, self.layers, path.data_ptr(), num_accepted.data_ptr(), next_token.data_ptr(), new_len.data_ptr(),
+            self.batch, self.nodes, self.num_kv_groups, self.head_dim, self.max_ctx, *kds, *vds, _lib.raw_stream(dev)))
         return path, num_accepted, next_token, new_len
 
 
@@ -785,22 +817,23 @@ class TokenLogProbs:
         return spec
 
     def __call__(self, logits, tokens, logprob, entropy=None, top_logprob=None, top_index=None, lse=None):
-        f32 = torch.float32
-        _check_arg("logits", logits, (self.rows, self.vocab), self.dtype, contiguous=False)
-        if self.vocab > 1 and logits.stride(1) != 1 or self.rows > 1 and logits.stride(0) < self.vocab:
+        dev, f32, row, top = _current_device(logits), torch.float32, (self.rows,), (self.rows, self.num_top)
+        _check_arg("logits", logits, (self.rows, self.vocab), self.dtype, dev, False)
+        ld = logits.stride(0) if self.rows > 1 else self.vocab
+        if self.vocab > 1 and logits.stride(1) != 1 or ld < self.vocab:
             raise ValueError("logits: rows must be contiguous and must not overlap")
-        _check_arg("tokens", tokens, (self.rows,), torch.int32)
-        _check_arg("logprob", logprob, (self.rows,), f32)
-        for nm, t in (("entropy", entropy), ("lse", lse)):
-            if t is not None:
-                _check_arg(nm, t, (self.rows,), f32)
+        _check_arg("tokens", tokens, row, torch.int32, dev)
+        _check_arg("logprob", logprob, row, f32, dev)
+        if entropy is not None:
+            _check_arg("entropy", entropy, row, f32, dev)
+        if lse is not None:
+            _check_arg("lse", lse, row, f32, dev)
         if (self.num_top > 0) != (top_logprob is not None) or (self.num_top > 0) != (top_index is not None):
             raise ValueError("top_logprob and top_index go with num_top > 0")
         if self.num_top:
-            _check_arg("top_logprob", top_logprob, (self.rows, self.num_top), f32)
-            _check_arg("top_index", top_index, (self.rows, self.num_top), torch.int32)
-        p = _lib.ptr
-        _lib.call("t2b_token_logprobs", p(logits), _lib.DTYPE[self.dtype], self.rows, self.vocab,
-                  logits.stride(0) if self.rows > 1 else self.vocab, p(tokens), p(logprob), p(entropy), p(lse),
-                  self.num_top, p(top_logprob), p(top_index), _lib.stream())
+            _check_arg("top_logprob", top_logprob, top, f32, dev)
+            _check_arg("top_index", top_index, top, torch.int32, dev)
+        _lib.check("t2b_token_logprobs", _lib.load().t2b_token_logprobs(
+            logits.data_ptr(), _lib.DTYPE[self.dtype], self.rows, self.vocab, ld, tokens.data_ptr(), logprob.data_ptr(),
+            _addr(entropy), _addr(lse), self.num_top, _addr(top_logprob), _addr(top_index), _lib.raw_stream(dev)))
         return logprob
