@@ -29,6 +29,7 @@ written by the qkv epilogue, so no per-layer host copy remains.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import numpy as np
@@ -90,6 +91,28 @@ def load_layer(layer: dict, cfg: QuantizedQwenConfig, device="cuda") -> LayerWei
         q_norm=bf(layer.get("q_norm")) if cfg.qk_norm else None,
         k_norm=bf(layer.get("k_norm")) if cfg.qk_norm else None,
     )
+
+
+@dataclass
+class PromptScores:
+    """What the model made of each prompt (``DecodeEngine.prefill_packed(score=True)``),
+    the prompts' positions one after the other (``lengths``): ``logprob[i]`` of
+    the token that follows position i in its prompt (NaN at a prompt's last
+    position), ``entropy[i]`` and the ``top_*[i]`` alternatives of the
+    distribution there.  ``of(b)`` gives prompt b's share."""
+
+    lengths: list
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: torch.Tensor | None
+    top_index: torch.Tensor | None
+
+    def of(self, b: int) -> dict:
+        at = sum(self.lengths[:b])
+        end = at + self.lengths[b]
+        return {"logprob": self.logprob[at:end - 1], "entropy": self.entropy[at:end],
+                "top_logprob": None if self.top_logprob is None else self.top_logprob[at:end],
+                "top_index": None if self.top_index is None else self.top_index[at:end]}
 
 
 class DecodeEngine:
@@ -401,7 +424,21 @@ class DecodeEngine:
         """One chunk: tokens ``c0 .. c0+n-1`` of every sequence (rows ``b*n + i``
         of ``pf``, already holding tokens / pos / seq) through all layers."""
         cfg, B = self.cfg, self.B
-        M = B * n
+        p = _lib.ptr
+
+        def attention(li):
+            _lib.check("t2b_prefill_attention", _lib.lib().t2b_prefill_attention(
+                p(pf["q"]), p(self.k_cache[li]), p(self.v_cache[li]), p(pf["attn"]), _lib.DTYPE[_lib.ACT], B, n, c0,
+                cfg.n_heads, cfg.n_kv_groups, cfg.head_dim, self.max_ctx, st))
+
+        self._enqueue_rows(pf, B * n, st, self.angles, self.k_cache, self.v_cache, B, self.max_ctx, attention)
+
+    def _enqueue_rows(self, pf: dict, M: int, st, angles, k_out, v_out, n_seq: int, max_ctx: int, attention) -> None:
+        """``M`` rows of ``pf`` (tokens / pos / seq) through all layers: row m's
+        K/V go to ``k_out[layer]`` / ``v_out[layer]`` ``[n_seq][n_kv][max_ctx][hd]``
+        at sequence ``seq[m]``, position ``pos[m]`` (whose RoPE row of ``angles``
+        it takes), and ``attention(layer)`` enqueues q -> attn."""
+        cfg = self.cfg
         H, hd, nq, nkv = cfg.emb_dim, cfg.head_dim, cfg.n_heads, cfg.n_kv_groups
         L = _lib.lib()
         p = _lib.ptr
@@ -417,12 +454,9 @@ class DecodeEngine:
         for li, lw in enumerate(self.layers):
             _lib.check("t2b_qkv_norm_rope_kvwrite_seq", L.t2b_qkv_norm_rope_kvwrite_seq(
                 p(lw.qkv.qw), p(lw.qkv.meta), lw.qkv.fmt, p(xw), p(sa), cfg.rms_norm_eps, p(lw.q_norm), p(lw.k_norm),
-                p(self.angles), p(pf["pos"]), p(pf["seq"]), B, p(pf["q"]), p(self.k_cache[li]), p(self.v_cache[li]),
-                p(sb), M, H, nq, nkv, hd, self.max_ctx, *ws("qkv"), st))
-            _lib.check("t2b_prefill_attention", L.t2b_prefill_attention(
-                p(pf["q"]), p(self.k_cache[li]), p(self.v_cache[li]), p(pf["attn"]), _lib.DTYPE[_lib.ACT], B, n, c0,
-                nq, nkv, hd,
-                self.max_ctx, st))
+                p(angles), p(pf["pos"]), p(pf["seq"]), n_seq, p(pf["q"]), p(k_out[li]), p(v_out[li]),
+                p(sb), M, H, nq, nkv, hd, max_ctx, *ws("qkv"), st))
+            attention(li)
             _lib.check("t2b_oproj_residual", L.t2b_oproj_residual(
                 p(lw.o_proj.qw), p(lw.o_proj.meta), lw.o_proj.fmt, p(pf["attn"]), p(x), p(sb), p(lw.post_attention_layernorm),
                 p(xw), M, H, cfg.q_dim, *ws("o"), st))
@@ -511,6 +545,236 @@ class DecodeEngine:
             self.run_step()
         self.tokens.copy_(self.next_tokens)
         self.pos.fill_(P)
+
+    # -- packed prefill, prompt scoring and draft-tree decoding ---------------
+    HEAD_ROWS = 256          # rows per lm_head call (t2b_lm_head_argmax takes up to 256)
+
+    def _varlen_ws(self):
+        """Workspace of the packed and tree attention (kept for reuse)."""
+        if getattr(self, "_va_ws", None) is None:
+            n = _lib.load().t2b_varlen_attention_workspace_bytes(self.cfg.head_dim)
+            self._va_ws = (torch.empty(n, dtype=torch.uint8, device=self.device), n)
+        t, n = self._va_ws
+        return _lib.ptr(t), n
+
+    def _head_buffers(self, logits: bool) -> dict:
+        """Buffers of a head over up to ``HEAD_ROWS`` rows (kept for reuse)."""
+        hb = getattr(self, "_hb", None)
+        if hb is None:
+            cfg, R, dev, L = self.cfg, self.HEAD_ROWS, self.device, _lib.load()
+            hb = {"xn": torch.zeros(R, cfg.emb_dim, dtype=torch.float16, device=dev), "logits": None}
+            sizes = {"lm": L.t2b_lm_head_argmax_workspace_bytes(R)} if self.lm_w4 is None else \
+                {"lm": L.t2b_w4a16_gemm_workspace_bytes(R, cfg.vocab_size, cfg.emb_dim),
+                 "am": L.t2b_argmax_workspace_bytes(R, cfg.vocab_size)}
+            hb["ws"] = {k: (torch.zeros(max(v, 256), dtype=torch.uint8, device=dev), max(v, 256))
+                        for k, v in sizes.items()}
+            self._hb = hb
+        if hb["logits"] is None and (logits or self.lm_w4 is not None):
+            hb["logits"] = torch.zeros(self.HEAD_ROWS, self.cfg.vocab_size, dtype=torch.float32, device=self.device)
+        return hb
+
+    def _enqueue_head_rows(self, x, ssq, rows: int, idx, st, logits: bool = False):
+        """Final RMSNorm and lm_head of ``rows`` <= ``HEAD_ROWS`` rows of a
+        residual stream: greedy ids into ``idx``, and the fp32 logits (returned) if asked for."""
+        cfg, hb, L, p = self.cfg, self._head_buffers(logits), _lib.lib(), _lib.ptr
+        f16 = _lib.DTYPE[torch.float16]
+
+        def ws(k):
+            t, nb = hb["ws"][k]
+            return p(t), nb
+
+        _lib.check("t2b_rms_norm_rows", L.t2b_rms_norm_rows(p(x), p(ssq), p(self.final_norm), cfg.rms_norm_eps,
+                                                            p(hb["xn"]), f16, rows, cfg.emb_dim, st))
+        if self.lm_w4 is None:
+            _lib.check("t2b_lm_head_argmax", L.t2b_lm_head_argmax(
+                p(hb["xn"]), p(self.lm_head), f16, rows, cfg.emb_dim, cfg.vocab_size, p(idx), None,
+                p(hb["logits"]) if logits else None, *ws("lm"), st))
+        else:
+            _lib.check("t2b_w4a16_gemm", L.t2b_w4a16_gemm(
+                p(self.lm_w4.qw), p(self.lm_w4.meta), self.lm_w4.fmt, p(hb["xn"]), f16,
+                p(hb["logits"]), _lib.DTYPE[torch.float32], rows, cfg.vocab_size, cfg.emb_dim,
+                32 if self.lm_w4.fmt == W.WFMT_Q4NX else 128, *ws("lm"), st))
+            _lib.check("t2b_argmax_rows", L.t2b_argmax_rows(
+                p(hb["logits"]), _lib.DTYPE[torch.float32], rows, cfg.vocab_size, cfg.vocab_size, p(idx), *ws("am"), st))
+        return hb["logits"][:rows] if logits else None
+
+    def _packed_prompts(self, prompts) -> list[np.ndarray]:
+        got = [np.asarray(t.cpu() if isinstance(t, torch.Tensor) else t).reshape(-1) for t in prompts]
+        if len(got) != self.B:
+            raise ValueError(f"{len(got)} prompts for an engine of {self.B} rows")
+        for t in got:
+            if not 1 <= len(t) <= self.max_ctx:
+                raise ValueError(f"prompt length {len(t)} outside 1..{self.max_ctx}")
+            if not np.issubdtype(t.dtype, np.integer) or t.min() < 0 or t.max() >= self.cfg.vocab_size:
+                raise ValueError(f"token ids must be integers in [0, {self.cfg.vocab_size})")
+        return got
+
+    def prefill_packed(self, prompts, score: bool = False, num_top: int = 0, chunk_rows: int | None = None):
+        """Fill the KV caches from ``B`` prompts of any lengths, without padding:
+        the prompts' tokens lie one after the other, up to ``chunk_rows`` (default
+        ``PREFILL_ROWS``) per pass, every linear runs over exactly those rows and
+        attention is ``t2b_packed_attention`` over the cache rows.  Leaves the
+        engine as ``prefill`` does (next tokens, positions, ready to decode).
+
+        With ``score`` every position's distribution is evaluated as well and a
+        :class:`PromptScores` is returned: the log probability of each prompt
+        token after the first, the entropy at every position and the
+        ``num_top`` most likely next tokens there."""
+        from .operators import TokenLogProbs
+        ids = self._packed_prompts(prompts)
+        if not 0 <= num_top <= min(32, self.cfg.vocab_size):
+            raise ValueError("num_top must be in 0..min(32, vocab_size)")
+        if num_top and not score:
+            raise ValueError("num_top goes with score")
+        rows_max = chunk_rows or self.PREFILL_ROWS
+        if rows_max < 1:
+            raise ValueError("chunk_rows must be positive")
+        dev, B, cfg = self.device, self.B, self.cfg
+        lens = np.array([len(t) for t in ids])
+        total = int(lens.sum())
+        at = np.concatenate([[0], np.cumsum(lens)])
+        host = np.empty((4, total), np.int32)                 # token, position, cache row, next token of the prompt
+        host[0] = np.concatenate(ids)
+        host[1] = np.arange(total) - np.repeat(at[:-1], lens)
+        host[2] = np.repeat(np.arange(B), lens)
+        host[3, :-1] = host[0, 1:]
+        host[3, at[1:] - 1] = -1                              # no target behind a prompt's last token
+        rows = torch.from_numpy(host).to(dev)
+        C = min(rows_max, total)
+        pf = self._prefill_buffers(C)
+        starts, k_lens = [], []
+        for c0 in range(0, total, C):
+            c1 = min(c0 + C, total)
+            cut = np.clip(at, c0, c1)                         # the sequences' rows inside this pass
+            starts.append(cut - c0)
+            k_lens.append(cut[1:] - at[:-1])                  # keys in the cache after it (unused without rows)
+        starts = torch.from_numpy(np.stack(starts).astype(np.int32)).to(dev)
+        k_lens = torch.from_numpy(np.maximum(np.stack(k_lens), 0).astype(np.int32)).to(dev)
+        out = None
+        if score:
+            f32 = torch.float32
+            out = {"logprob": torch.empty(total, dtype=f32, device=dev), "entropy": torch.empty(total, dtype=f32, device=dev),
+                   "top_logprob": torch.empty(total, num_top, dtype=f32, device=dev) if num_top else None,
+                   "top_index": torch.empty(total, num_top, dtype=torch.int32, device=dev) if num_top else None}
+            picks = torch.empty(self.HEAD_ROWS, dtype=torch.int32, device=dev)
+        p, st = _lib.ptr, _lib.stream()
+        act, bf = _lib.DTYPE[_lib.ACT], _lib.DTYPE[torch.bfloat16]
+        nq, nkv, hd, ctx = cfg.n_heads, cfg.n_kv_groups, cfg.head_dim, self.max_ctx
+        scale, seq_stride = hd ** -0.5, nkv * ctx * hd
+        with _lib.status_word(self.err, st):
+            for ci, c0 in enumerate(range(0, total, C)):
+                M = min(C, total - c0)
+                for i, k in enumerate(("tokens", "pos", "seq")):
+                    pf[k][:M].copy_(rows[i, c0:c0 + M])
+
+                def attention(li):
+                    _lib.check("t2b_packed_attention", _lib.lib().t2b_packed_attention(
+                        p(pf["q"]), p(self.k_cache[li]), p(self.v_cache[li]), p(pf["attn"]), None, bf, act,
+                        p(starts[ci]), None, p(k_lens[ci]), B, M, B, ctx, nq, nkv, hd, nq * hd, hd, nq * hd, hd, hd,
+                        ctx * hd, seq_stride, hd, ctx * hd, seq_stride, scale, *self._varlen_ws(), st))
+
+                self._enqueue_rows(pf, M, st, self.angles, self.k_cache, self.v_cache, B, ctx, attention)
+                ends = np.nonzero((at[1:] > c0) & (at[1:] <= c0 + M))[0]          # prompts that end in this pass
+                if len(ends):
+                    dst = torch.from_numpy(ends).to(dev)
+                    src = torch.from_numpy(at[1:][ends] - 1 - c0).to(dev)
+                    self.x.index_copy_(0, dst, pf["x"].index_select(0, src))
+                    self.ssq_a.index_copy_(0, dst, pf["ssq_a"].index_select(0, src))
+                for r0 in range(0, M if score else 0, self.HEAD_ROWS):
+                    n, o = min(self.HEAD_ROWS, M - r0), c0 + r0
+                    logits = self._enqueue_head_rows(pf["x"][r0:], pf["ssq_a"][r0:], n, picks, st, logits=True)
+                    TokenLogProbs(rows=n, vocab=cfg.vocab_size, num_top=num_top)(
+                        logits, rows[3, o:o + n], out["logprob"][o:o + n], entropy=out["entropy"][o:o + n],
+                        top_logprob=out["top_logprob"][o:o + n] if num_top else None,
+                        top_index=out["top_index"][o:o + n] if num_top else None)
+            self._enqueue_head(st)
+        self.tokens.copy_(self.next_tokens)
+        self.pos.copy_(torch.from_numpy(lens.astype(np.int32)))
+        return None if out is None else PromptScores(lens.tolist(), **out)
+
+    def _tree_buffers(self, nodes: int) -> dict:
+        """Draft K/V and walk buffers for trees of ``nodes`` nodes (kept for reuse)."""
+        tb = getattr(self, "_tb", None)
+        if tb is None or tb["nodes"] != nodes:
+            cfg, dev, B, M, i32 = self.cfg, self.device, self.B, self.B * nodes, torch.int32
+            shape = (cfg.n_layers, cfg.n_kv_groups, M, cfg.head_dim)
+            words = (nodes + 63) // 64
+            tb = {"nodes": nodes, "k": torch.zeros(shape, dtype=torch.bfloat16, device=dev),
+                  "v": torch.zeros(shape, dtype=torch.bfloat16, device=dev),
+                  "rows": torch.arange(M, dtype=i32, device=dev), "predicted": torch.zeros(B, nodes, dtype=i32, device=dev),
+                  "tree": torch.zeros(3, B, nodes, dtype=i32, device=dev), "live": torch.zeros(B, dtype=i32, device=dev),
+                  "mask": torch.zeros(B, nodes, words, dtype=torch.int64, device=dev),
+                  "path": torch.zeros(B, nodes, dtype=i32, device=dev), "walk": torch.zeros(3, B, dtype=i32, device=dev)}
+            self._tb = tb
+        return tb
+
+    def decode_tree(self, tokens, parents, num_nodes=None):
+        """One speculative step: verify a tree of drafted tokens per row.
+
+        ``tokens`` / ``parents`` (host, ``[B, T]``, T <= 256): node 0 is the row's
+        pending token (``tokens`` after ``prefill`` or ``advance``), every other
+        node follows its parent, ``num_nodes`` (default T) of each row are live.
+        All nodes run through the model at once (``t2b_tree_attention`` over the
+        cache), and each row keeps the branch along which every drafted token is
+        the model's own greedy token: its K/V rows move into the cache
+        (``t2b_tree_commit``) and the row continues behind it.  A row without live
+        nodes, or without room in the cache, is left as it is.
+
+        Returns host int32 tensors ``(path [B, T], num_accepted [B], next_tokens
+        [B])``: the accepted nodes (-1 behind them; the row emitted the tokens of
+        ``path[1:num_accepted]`` and then ``next_tokens``)."""
+        from .operators import draft_tree
+        cfg, B, dev = self.cfg, self.B, self.device
+        tok = np.asarray(tokens.cpu() if isinstance(tokens, torch.Tensor) else tokens)
+        par = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
+        if tok.ndim != 2 or tok.shape[0] != B or tok.shape != par.shape or not 1 <= tok.shape[1] <= 256:
+            raise ValueError(f"decode_tree takes tokens and parents [{B}, nodes] with nodes in 1..256")
+        if not np.issubdtype(tok.dtype, np.integer) or tok.min() < 0 or tok.max() >= cfg.vocab_size:
+            raise ValueError(f"token ids must be integers in [0, {cfg.vocab_size})")
+        T = tok.shape[1]
+        mask, depth = draft_tree(par, num_nodes)
+        live = np.full(B, T) if num_nodes is None else np.asarray(num_nodes).reshape(-1)
+        M, tb, pf = B * T, self._tree_buffers(T), self._prefill_buffers(B * T)
+        tb["tree"].copy_(torch.from_numpy(np.stack([tok, par, depth.numpy()]).astype(np.int32)))
+        tb["live"].copy_(torch.from_numpy(live.astype(np.int32)))
+        tb["mask"].copy_(mask)
+        # A node's RoPE position is its row's context plus its depth, its K/V slot
+        # its own: the qkv kernel gets the nodes as positions 0 .. M-1 of one
+        # sequence and a table whose row m is the angle row of node m.
+        at = (self.pos[:, None] + tb["tree"][2]).clamp_(0, self.max_ctx - 1).reshape(-1)
+        angles = self.angles.index_select(0, at)
+        pf["tokens"][:M].copy_(tb["tree"][0].reshape(-1))
+        pf["pos"][:M].copy_(tb["rows"])
+        pf["seq"][:M].zero_()
+        p, st, L = _lib.ptr, _lib.stream(), _lib.lib()
+        act, bf = _lib.DTYPE[_lib.ACT], _lib.DTYPE[torch.bfloat16]
+        nq, nkv, hd, ctx = cfg.n_heads, cfg.n_kv_groups, cfg.head_dim, self.max_ctx
+        kd, vd, drafted = tb["k"], tb["v"], (T * hd, hd, M * hd)       # row, node and head strides of the drafts
+
+        def attention(li):
+            _lib.check("t2b_tree_attention", L.t2b_tree_attention(
+                p(pf["q"]), p(self.k_cache[li]), p(self.v_cache[li]), p(kd[li]), p(vd[li]), p(pf["attn"]), None, bf, act,
+                p(self.pos), p(tb["live"]), p(tb["mask"]), B, T, nq, nkv, hd, ctx, nq * hd, hd, nq * hd, hd, *drafted,
+                *drafted, hd ** -0.5, *self._varlen_ws(), st))
+
+        with _lib.status_word(self.err, st):
+            self._enqueue_rows(pf, M, st, angles, kd, vd, 1, M, attention)
+            flat = tb["predicted"].reshape(-1)
+            for r0 in range(0, M, self.HEAD_ROWS):
+                n = min(self.HEAD_ROWS, M - r0)
+                self._enqueue_head_rows(pf["x"][r0:], pf["ssq_a"][r0:], n, flat[r0:], st)
+            layers = [(ctypes.c_void_p * cfg.n_layers)(*(t.data_ptr() for t in ts))
+                      for ts in (kd.unbind(0), vd.unbind(0), self.k_cache, self.v_cache)]
+            count, following, length = tb["walk"]
+            _lib.check("t2b_tree_commit", L.t2b_tree_commit(
+                p(tb["tree"][0]), p(tb["tree"][1]), p(tb["predicted"]), p(self.pos), p(tb["live"]), *layers, cfg.n_layers,
+                p(tb["path"]), p(count), p(following), p(length), B, T, nkv, hd, ctx, *drafted, *drafted, st))
+        self.pos.copy_(length)
+        self.tokens.copy_(torch.where(count > 0, following, self.tokens))
+        self.next_tokens.copy_(self.tokens)
+        path, walk = tb["path"].cpu(), tb["walk"].cpu()
+        self.check_device_errors()
+        return path, walk[0].clone(), walk[1].clone()
 
     def generate(self, prompts: torch.Tensor, new_tokens: int, stepwise_prefill: bool = False,
                  lengths=None) -> torch.Tensor:
