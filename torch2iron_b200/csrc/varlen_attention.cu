@@ -10,13 +10,15 @@
 //
 // Work.  The qpg query heads of a kv head share its keys, so a tile is 128
 // MMA rows = 128 / qpg tokens x qpg heads, and an item two neighbouring tiles
-// of one (sequence, kv head).  An item's keys are blocks of 128, and one
-// (item, block) is a unit.  All units of the call form one list, which the
-// CTAs (one per SM) cut into equal ranges: prompts of any lengths, long
-// contexts with few rows and single tokens balance alike without the host
-// knowing a length.  An item cut between CTAs leaves fp32 partials (output,
-// maximum, sum) that a second kernel joins in a fixed order; items of up to
-// VA_SNAP blocks are not cut.
+// of one (sequence, kv head), or its last one.  An item's keys are blocks of
+// 128; a block counts one unit for one tile and two for two, an item VA_ITEM
+// units more (about what its start and end cost).  The units of the call form
+// one list, which the CTAs (one per SM) cut into equal ranges: prompts of any
+// lengths, long contexts with few rows and single tokens balance alike without
+// the host knowing a length.  An item cut between CTAs leaves fp32 partials
+// (output, maximum, sum) that a second kernel joins in a fixed order; items of
+// up to VA_SNAP blocks are not cut.  (24 ragged prompts: 276 us with blocks
+// alone counted, 174 us with the items' own cost.)
 //
 // CTA: two softmax groups of four warps, a TMA warp and an MMA warp.
 //   S_t = Q_t K^T     A, B from shared memory (128-byte swizzled TMA tiles)
@@ -59,9 +61,9 @@ constexpr int VA_THREADS = 640;         // 16 softmax warps, TMA, MMA, 2 that on
 // warpgroups take 104 and the fifth gives down to 64: 512 * 104 + 128 * 64 = 61440.
 constexpr int VA_REGS_SOFTMAX = 104, VA_REGS_OTHER = 64;
 constexpr int VA_WARP_TMA = 16, VA_WARP_MMA = 17;
-constexpr int VA_ITEM = 2;              // what an item costs beside its blocks, in blocks (see Work)
+constexpr int VA_ITEM = 4;              // units an item costs beside its blocks (see Work)
 constexpr int VA_SNAP = 8;              // items of up to this many blocks stay in one CTA
-constexpr int VA_MIN_UNITS = 3;         // units per CTA, at least
+constexpr int VA_MIN_UNITS = 5;         // units per CTA, at least
 constexpr float VA_HEAD = 7.f, VA_ROOM = 15.f;
 
 struct VaParams {
@@ -157,21 +159,26 @@ T2B_DEV uint32_t va_floor_sum(uint32_t n, uint32_t a, uint32_t b) {
   }
   return sum;
 }
-// Blocks of pairs 0 .. k - 1 of a sequence, in closed form: pairs that see at
-// most one block, then a line's blocks, then pairs that see every key.  (The
-// sequences of a long prompt have hundreds of pairs; a loop over them cost
-// 14 us at the start of a 1.9 ms call.)
+// Units of pair p of a sequence, for one kv head.
 template <bool TREE>
-T2B_DEV uint32_t va_blocks_before(const VaSeq& q, int tpt, int pairs, int k) {
-  if (TREE) return k ? (uint32_t)k * va_tile_blocks<TREE>(q, tpt, 0, 0) : 0u;
-  uint32_t sum = 0;
-  if (k == pairs && k > 0) sum = va_tile_blocks<TREE>(q, tpt, --k, 1);   // the last pair may be short
+T2B_DEV uint32_t va_units(const VaSeq& q, int tpt, int p) {
+  return va_tile_blocks<TREE>(q, tpt, p, 1) * (q.n > (2 * p + 1) * tpt ? 2 : 1) + VA_ITEM;
+}
+// Units of pairs 0 .. k - 1, in closed form: pairs that see at most one block,
+// then a line's blocks, then pairs that see every key.  (The sequences of a
+// long prompt have hundreds of pairs; a loop over them cost 14 us at the start
+// of a call.)
+template <bool TREE>
+T2B_DEV uint32_t va_units_before(const VaSeq& q, int tpt, int pairs, int k) {
+  uint32_t last = 0;
+  if (k == pairs && k > 0) last = va_units<TREE>(q, tpt, --k);   // only the last pair may be short or alone
+  if (TREE) return last + (k ? (uint32_t)k * va_units<TREE>(q, tpt, 0) : 0u);
   const int t = 2 * tpt;                                // pair p sees min(off + (p + 1) t, avail) keys
   const int one = VA_ROWS - q.off < t ? 0 : min(k, va_div(VA_ROWS - q.off, t));
   const int rise = q.avail - q.off <= 0 ? one : max(one, min(k, va_div(q.avail - q.off + t - 1, t) - 1));
-  sum += one + (k - rise) * max(1, va_blocks(q.avail));
-  if (rise > one) sum += va_floor_sum(rise - one, t, q.off + (one + 1) * t + VA_ROWS - 1);
-  return sum;
+  uint32_t blocks = one + (k - rise) * max(1, va_blocks(q.avail));
+  if (rise > one) blocks += va_floor_sum(rise - one, t, q.off + (one + 1) * t + VA_ROWS - 1);
+  return last + 2 * blocks + k * VA_ITEM;
 }
 
 // A position in the list of units: block b of item (s, p, g).
@@ -208,9 +215,10 @@ struct VaWalk {
     }
     dual = q.n > (2 * p + 1) * P.tpt;
     nb = va_tile_blocks<TREE>(q, P.tpt, p, dual ? 1 : 0);
-    n = min(left, nb - b0);
+    const int w = dual ? 2 : 1;
+    n = min(left / w, nb - b0);
     n0 = dual ? min(n, va_tile_blocks<TREE>(q, P.tpt, p, 0) - b0) : n;
-    left -= n + (b0 + n == nb ? VA_ITEM : 0);
+    left -= n * w + (b0 + n == nb ? VA_ITEM : 0);
     return true;
   }
 };
@@ -427,7 +435,7 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
     if (s >= P.n_seqs) return 0;
     mine = va_seq<TREE>(P, s);
     const int pairs = va_pairs(mine, P.tpt);
-    return (va_blocks_before<TREE>(mine, P.tpt, pairs, pairs) + pairs * VA_ITEM) * P.n_kv;
+    return va_units_before<TREE>(mine, P.tpt, pairs, pairs) * P.n_kv;
   };
   // inclusive sum of one value per thread over the block, and the block's total
   auto block_scan = [&](uint32_t v, uint32_t& sum) -> uint32_t {
@@ -489,17 +497,16 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
       const VaSeq q = va_seq<TREE>(P, s);
       const int pairs = va_pairs(q, P.tpt), step = (pairs + VA_THREADS / 2 - 1) / (VA_THREADS / 2);
       int p = t * step;
-      uint32_t at = p < pairs ? (va_blocks_before<TREE>(q, P.tpt, pairs, p) + p * VA_ITEM) * P.n_kv : 0u;
+      uint32_t at = p < pairs ? va_units_before<TREE>(q, P.tpt, pairs, p) * P.n_kv : 0u;
       for (const int last = min(pairs, p + step); p < last; ++p) {
-        const uint32_t nb = va_tile_blocks<TREE>(q, P.tpt, p, 1), w = nb + VA_ITEM;
+        const uint32_t w = va_units<TREE>(q, P.tpt, p);
         if (u >= at && u - at < w * P.n_kv) {   // one thread's
-          int g = (u - at) / w, b = (u - at) - g * w, np = p;
-          uint32_t place = cut[i];
-          if (b >= (int)nb || (nb <= VA_SNAP && b)) {
-            if (2 * b < (int)w) {
-              place -= b;
-            } else {   // up to the next item
-              place += w - b;
+          const int bw = q.n > (2 * p + 1) * P.tpt ? 2 : 1, nb = (int)(w - VA_ITEM) / bw;
+          int g = (u - at) / w, rest = (u - at) - g * w, b = rest / bw, np = p;
+          uint32_t place = cut[i] - rest;       // the item's start
+          if (b >= nb || (nb <= VA_SNAP && rest)) {
+            if (2 * rest >= (int)w) {           // up to the next item
+              place += w;
               if (++g == P.n_kv) {
                 g = 0;
                 ++np;
@@ -507,6 +514,7 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
             }
             b = 0;
           }
+          place += b * bw;
           s_range[i] = place;
           if (i == 0) {
             int ns = s;
@@ -951,6 +959,8 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
   }
 }
 
+constexpr int VA_JOIN_Y = 8;            // blocks per item that was cut
+
 // Joins the partials of the items that were cut: block (c, y) takes a few rows
 // of the item that begins in CTA c and ends in a later one.  The pieces are
 // CTA c's last and the first of the CTAs after it, joined in that order.  The
@@ -964,10 +974,7 @@ __global__ void __launch_bounds__(256) varlen_join_kernel(const __grid_constant_
   const int4 tail = P.head[2 * c];
   if (!tail.w) return;
   const VaSeq q = va_seq<TREE>(P, tail.x);
-  const int row = blockIdx.y * ROWS + threadIdx.x / LPR, col = (threadIdx.x % LPR) * 4;
-  const int tile = row / VA_ROWS, in_tile = row % VA_ROWS;
-  const int tok = in_tile / P.qpg, i_row = (2 * tail.y + tile) * P.tpt + tok;
-  if (tok >= P.tpt || i_row >= q.n) return;
+  const int col = (threadIdx.x % LPR) * 4;
   int last = c;
   for (;;) {
     if (++last >= grid) return;   // (a CTA gave up: the status word says so)
@@ -975,6 +982,10 @@ __global__ void __launch_bounds__(256) varlen_join_kernel(const __grid_constant_
     if (!f.x) return;
     if (f.y) break;
   }
+  for (int row = blockIdx.y * ROWS + threadIdx.x / LPR; row < 2 * VA_ROWS; row += ROWS * VA_JOIN_Y) {
+  const int tile = row / VA_ROWS, in_tile = row % VA_ROWS;
+  const int tok = in_tile / P.qpg, i_row = (2 * tail.y + tile) * P.tpt + tok;
+  if (tok >= P.tpt || i_row >= q.n) continue;
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int j0 = c; j0 <= last; j0 += BATCH) {
@@ -1012,6 +1023,7 @@ __global__ void __launch_bounds__(256) varlen_join_kernel(const __grid_constant_
   uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + r * P.o_row + h * P.o_head + col);
   *dst = make_uint2(va_pack_out(o.x * inv, o.y * inv, P.out_f16), va_pack_out(o.z * inv, o.w * inv, P.out_f16));
   if (P.lse && col == 0) P.lse[r * P.n_heads + h] = (m + __log2f(l)) * 0.6931471805599453f;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1057,7 +1069,7 @@ static int va_launch_t(VaParams& P, int grid, bool join, cudaStream_t st) {
   if (allow_smem(kern, VaGeom<HD>::BYTES) != T2B_OK) return T2B_ERR_LAUNCH;
   const int rc = launch_pdl(kern, dim3(grid), dim3(VA_THREADS), (size_t)VaGeom<HD>::BYTES, st, P);
   if (rc != T2B_OK || !join) return rc;
-  return launch_pdl(varlen_join_kernel<HD, TREE>, dim3(grid, 256 * (HD / 4) / 256), dim3(256), 0, st, P, grid);
+  return launch_pdl(varlen_join_kernel<HD, TREE>, dim3(grid, VA_JOIN_Y), dim3(256), 0, st, P, grid);
 }
 
 // max_blocks: no item has more blocks of keys; pairs: no more (sequence, pair of tiles).
@@ -1075,7 +1087,7 @@ static int va_launch(VaParams& P, int hd, bool f16, const void* q, size_t q_row,
   int dev = 0, sms = VA_MAX_CTAS;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return T2B_ERR_LAUNCH;
-  const long long units = pairs * (max_blocks + VA_ITEM) * P.n_kv;
+  const long long units = pairs * (2 * max_blocks + VA_ITEM) * P.n_kv;
   if (units > 0x7fffffffll) return T2B_ERR_SHAPE;
   const int grid = (int)std::max(1ll, std::min<long long>({units / VA_MIN_UNITS, sms, VA_MAX_CTAS}));
   const bool join = grid > 1 && max_blocks > VA_SNAP;

@@ -32,8 +32,8 @@ NPU; ``W4A16GEMV`` consumes the reference's own ``qparam`` rows unchanged.
 
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 from dataclasses import dataclass, field
 from typing import NamedTuple
 
@@ -431,23 +431,28 @@ def _check_arg(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, dev
 
 def _current_device(t: torch.Tensor) -> int:
     """The current device's index (-2, which no tensor has, where there is none)."""
-    return torch.cuda.current_device() if t.is_cuda else -2
+    return torch._C._cuda_getDevice() if t.is_cuda else -2
 
 
 def _strides(name: str, t: torch.Tensor) -> list[int]:
     """Element strides of every axis but the last (contiguous) one, as the
     kernels take them: nonzero multiples of 8 on a 16-byte aligned base."""
-    shape, strides = t.shape, t.stride()
-    if strides[-1] != 1 and shape[-1] > 1:
+    *out, inner = t.stride()
+    low = 0
+    for s in out:
+        low |= s
+    if inner == 1 and low % 8 == 0 and t.data_ptr() % 16 == 0 and 0 not in out:
+        return out
+    shape = t.shape
+    if inner != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: the last axis must be contiguous")
     if t.data_ptr() % 16:
         raise ValueError(f"{name}: must start on a 16-byte boundary")
-    out = []
-    for i in range(len(shape) - 1):
-        s = strides[i] if shape[i] > 1 else 8          # an axis of one has no stride
-        if s % 8 or s <= 0:
-            raise ValueError(f"{name}: strides {strides} must be nonzero multiples of 8 elements")
-        out.append(s)
+    for i, s in enumerate(out):
+        if shape[i] == 1:
+            out[i] = 8                                 # an axis of one has no stride
+        elif s % 8 or s == 0:
+            raise ValueError(f"{name}: strides {t.stride()} must be nonzero multiples of 8 elements")
     return out
 
 
@@ -736,14 +741,14 @@ class DraftTreeCommit:
                 ArgSpec("out", (self.batch,), i32)]
 
     def _layers(self, name: str, ts, shape: tuple, dev: int, contiguous: bool):
-        """Host array of the layers' device pointers, and the strides they share."""
+        """Host array of the layers' device pointers (64 bits each), and the strides they share."""
         if isinstance(ts, torch.Tensor):
             _check_arg(name, ts, (self.layers, *shape), self.dtype, dev, False)
-            strides = _strides(name, ts)
-            step, base = strides[0] * ts.element_size(), ts.data_ptr()
-            at, strides = range(base, base + step * self.layers, step), strides[1:]
-            if contiguous and not ts[0].is_contiguous():
+            step, *strides = _strides(name, ts)
+            if contiguous and not ts.is_contiguous() and not ts[0].is_contiguous():
                 raise ValueError(f"{name}: must be contiguous")
+            base, step = ts.data_ptr(), step * 2
+            at = array("Q", range(base, base + step * self.layers, step))
         else:
             if len(ts) != self.layers:
                 raise ValueError(f"{name}: expected {self.layers} layers, got {len(ts)}")
@@ -753,10 +758,10 @@ class DraftTreeCommit:
                 if t.stride() != layout:
                     raise ValueError(f"{name}: the layers' strides differ")
             strides = _strides(name, ts[0])
-            at = [t.data_ptr() for t in ts]
+            at = array("Q", [t.data_ptr() for t in ts])
             if any(a % 16 for a in at):
                 raise ValueError(f"{name}: must start on a 16-byte boundary")
-        return (ctypes.c_void_p * self.layers)(*at), strides
+        return at, strides
 
     def __call__(self, tokens, parents, predicted, ctx_len, k_drafts, v_drafts, k_caches, v_caches, path, num_accepted,
                  next_token, new_len, num_nodes=None):
@@ -778,9 +783,10 @@ class DraftTreeCommit:
         kc, _ = self._layers("k_caches", k_caches, cache, dev, True)
         vc, _ = self._layers("v_caches", v_caches, cache, dev, True)
         _lib.check("t2b_tree_commit", _lib.load().t2b_tree_commit(
-            tokens.data_ptr(), parents.data_ptr(), predicted.data_ptr(), ctx_len.data_ptr(), _addr(num_nodes), kd, vd, kc,
-            vc, self.layers, path.data_ptr(), num_accepted.data_ptr(), next_token.data_ptr(), new_len.data_ptr(),
-            self.batch, self.nodes, self.num_kv_groups, self.head_dim, self.max_ctx, *kds, *vds, _lib.raw_stream(dev)))
+            tokens.data_ptr(), parents.data_ptr(), predicted.data_ptr(), ctx_len.data_ptr(), _addr(num_nodes),
+            *(a.buffer_info()[0] for a in (kd, vd, kc, vc)), self.layers, path.data_ptr(), num_accepted.data_ptr(),
+            next_token.data_ptr(), new_len.data_ptr(), self.batch, self.nodes, self.num_kv_groups, self.head_dim,
+            self.max_ctx, *kds, *vds, _lib.raw_stream(dev)))
         return path, num_accepted, next_token, new_len
 
 
