@@ -90,11 +90,11 @@ T2B_DEV LpSum lp_rescale(LpSum a, float m) {
   const float c = lp_ex2(d * LP_LOG2E);
   return {m, a.s * c, (a.z + a.s * d) * c};
 }
-T2B_DEV LpSum lp_join(LpSum a, LpSum b) {
-  const float m = fmaxf(a.m, b.m);
-  a = lp_rescale(a, m);
-  b = lp_rescale(b, m);
-  return {m, a.s + b.s, a.z + b.z};
+// The lanes' sums joined in lane order's butterfly: the maximum first, then
+// each lane's sums are rescaled once and added.
+T2B_DEV LpSum lp_warp_join(LpSum a) {
+  a = lp_rescale(a, warp_max(a.m));
+  return {a.m, warp_sum(a.s), warp_sum(a.z)};
 }
 
 template <typename T>
@@ -342,19 +342,12 @@ __global__ void __launch_bounds__(LP_THREADS, 3) token_logprobs_kernel(const LpP
     }
   }
   // ---- the CTA's sums, in a fixed order ----
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    LpSum b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.z = __shfl_xor_sync(0xffffffffu, a.z, o);
-    a = lp_join(a, b);
-  }
+  a = lp_warp_join(a);
   if ((tid & 31) == 0) S.sum[tid >> 5] = a;
   __syncthreads();
-  a = S.sum[0];
-#pragma unroll
-  for (int w = 1; w < LP_THREADS / 32; ++w) a = lp_join(a, S.sum[w]);
+  const int lane = tid & 31;
+  a = lane < LP_THREADS / 32 ? S.sum[lane] : LpSum{-INFINITY, 0.f, 0.f};
+  a = lp_warp_join(a);
   __syncthreads();
   if (K) lp_cut(S, K);
 
@@ -364,14 +357,23 @@ __global__ void __launch_bounds__(LP_THREADS, 3) token_logprobs_kernel(const LpP
     if (K && tid < K && tid >= S.n) S.list[tid] = 0;
     cluster_sync();
     if (split == 0) {
-      u64 got = 0;
-      const int from = K ? tid / K : 0;
-      if (K && from > 0 && from < P.splits) got = lp_peer_u64(&S.list[tid - from * K], from);
-      for (int i = 1; i < P.splits; ++i)
-        a = lp_join(a, {lp_peer_f32(&S.sum[0].m, i), lp_peer_f32(&S.sum[0].s, i), lp_peer_f32(&S.sum[0].z, i)});
+      const int from = K ? tid / K : P.splits;   // thread: place tid % K of range `from`
+      u64 key = 0;
+      if (from < P.splits) key = from ? lp_peer_u64(&S.list[tid - from * K], from) : S.list[tid];
+      LpSum b = {-INFINITY, 0.f, 0.f};
+      if (lane < P.splits)
+        b = {lp_peer_f32(&S.sum[0].m, lane), lp_peer_f32(&S.sum[0].s, lane), lp_peer_f32(&S.sum[0].z, lane)};
+      a = lp_warp_join(b);
       if (K) {
-        if (from > 0 && from < P.splits) S.list[tid] = got;   // places K.. on: this CTA's own stay first
-        if (tid == 0) S.n = P.splits * K;
+        // the ranges' keys are in order: at least K of all reach the least of
+        // their ceil(K / splits)-th ones, and only those are ranked
+        const int deep = (K + P.splits - 1) / P.splits - 1;
+        if (from < P.splits && tid - from * K == deep) S.group[from] = key;
+        if (tid == 0) S.n = 0;
+        __syncthreads();
+        u64 bound = S.group[0];
+        for (int i = 1; i < P.splits; ++i) bound = S.group[i] < bound ? S.group[i] : bound;
+        if (key && key >= bound) S.list[atomicAdd(&S.n, 1)] = key;
         __syncthreads();
         lp_cut(S, K);
       }
