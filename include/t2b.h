@@ -422,7 +422,9 @@ T2B_API int t2b_argmax_rows(const void* logits, int dtype, int M, int V, int ld,
  * scale > 0 multiplies q . k.  lse (may be NULL) is fp32 [rows][n_heads], the
  * natural log of the softmax sum.  A row that sees no key gets out = 0 and
  * lse = -inf.  Values of K and V that no row of the call sees may be anything,
- * infinities and NaN among them.  The lengths, starts and masks are read on
+ * infinities and NaN among them; so may a K value in the rows that do not see
+ * its key.  An infinity or NaN in a V value that some row sees may reach the
+ * other rows of its sequence too (0 times it is not 0).  The lengths, starts and masks are read on
  * the device; what lies outside the given extents is ignored (clamped), and
  * output rows that belong to no sequence or to no live node are not written.
  * The workspace (t2b_varlen_attention_workspace_bytes) needs no

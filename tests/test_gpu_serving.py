@@ -327,6 +327,51 @@ def test_tree_rows_that_see_nothing():
     check_tree(2, 6, [0, 40], (4, 2, 64), empty_row=True)
 
 
+def test_tree_nodes_that_no_mask_names_may_hold_anything():
+    """A padded batch without num_nodes: unused nodes have empty masks and uninitialised K/V."""
+    g, B, T, nh, nkv, hd, ctx = gen(40), 2, 70, 4, 2, 128, 100
+    used = [[0, 1, 5, 69], [0, 40, 66]]
+    q, kc, vc = randn(g, B, T, nh, hd), randn(g, B, nkv, 128, hd), randn(g, B, nkv, 128, hd)
+    kd, vd = randn(g, B, T, nkv, hd), randn(g, B, T, nkv, hd)
+    bits = torch.zeros(B, T, T, dtype=torch.bool)
+    for b in range(B):
+        for i in used[b]:
+            for j in used[b]:
+                bits[b, i, j] = j <= i
+        idle = [j for j in range(T) if j not in used[b]]
+        kd[b, idle], vd[b, idle] = math.nan, math.inf
+    packed = np.packbits(np.pad(bits.numpy(), ((0, 0), (0, 0), (0, 128 - T))), axis=2, bitorder="little").view("<i8")
+    op = DraftTreeAttention(batch=B, nodes=T, max_ctx=128, num_kv_groups=nkv, q_heads_per_group=2, head_dim=hd)
+    out, lse = torch.empty_like(q), torch.empty(B, T, nh, device="cuda")
+    op(q, kc, vc, kd, vd, ints([ctx, 0]), torch.from_numpy(packed.copy()).cuda(), out, lse=lse)
+    for b, c in enumerate((ctx, 0)):
+        k, v = (torch.cat([x[b, :, :c].transpose(0, 1), d[b]]) for x, d in ((kc, kd), (vc, vd)))
+        seen = torch.cat([torch.ones(T, c, dtype=torch.bool), bits[b]], 1)
+        assert_attention(out[b], lse[b], attention_rows(q[b], k, v, seen, op.scale))
+
+
+def test_packed_infinite_and_nan_keys_stay_with_the_rows_that_see_them():
+    g, n, hd = gen(41), 200, 64
+    q, k, v = randn(g, n, 2, hd), randn(g, n, 1, hd), randn(g, n, 1, hd)
+    k[150] = math.nan
+    out = torch.empty_like(q)
+    op = PackedAttention(tokens=n, num_seqs=1, num_kv_groups=1, q_heads_per_group=2, head_dim=hd)
+    op(q, k, v, ints([0, n]), out)
+    seen = torch.arange(150)[None] <= torch.arange(150)[:, None]
+    assert_attention(out[:150], None, attention_rows(q[:150], k[:150], v[:150], seen, op.scale))
+    assert torch.isnan(out[150:]).all()
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    from torch2iron_b200 import operators
+    op = TokenLogProbs(rows=1, vocab=4)
+    args = (torch.zeros(1, 4, device="cuda"), ints([0]), torch.zeros(1, device="cuda"))
+    op(*args)
+    monkeypatch.setattr(operators, "_current_device", lambda t: 1)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        op(*args)
+
+
 def test_tree_head_major_drafts_and_full_cache():
     check_tree(3, 17, [128, 64, 128], (8, 2, 64), max_ctx=128, head_major=True)
 

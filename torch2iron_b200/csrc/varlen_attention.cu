@@ -20,7 +20,7 @@
 // up to VA_SNAP blocks are not cut.  (24 ragged prompts: 276 us with blocks
 // alone counted, 174 us with the items' own cost.)
 //
-// CTA: two softmax groups of four warps, a TMA warp and an MMA warp.
+// CTA: two softmax groups of eight warps, a TMA warp and an MMA warp.
 //   S_t = Q_t K^T     A, B from shared memory (128-byte swizzled TMA tiles)
 //   P_t = 2^(S_t c - m)    TMEM -> registers -> TMEM, 16 bits, over S_t
 //   O_t += P_t V      A from TMEM, B = V as loaded (MN-major)
@@ -46,6 +46,7 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "t2b_common.cuh"
 #include "launch.cuh"
@@ -208,7 +209,7 @@ struct VaWalk {
       if (++p == va_pairs(q, P.tpt)) {
         p = 0;
         do {
-          ++s;
+          s = min(s + 1, P.n_seqs - 1);   // (the bound acts only where the lengths changed under the call)
           q = va_seq<TREE>(P, s);
         } while (q.n == 0 && s + 1 < P.n_seqs);
       }
@@ -592,113 +593,154 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
       P.head[2 * c + 1] = first;
     }
   } else if (warp == VA_WARP_MMA) {
-    // ---- MMA issuer (one lane; the others help to clear V rows) ----
+    // ---- MMA issuer (one lane; the others help to clear V rows).  It shares its
+    //      scheduler with four softmax warps, so every instruction here delays
+    //      the tensor pipe: descriptors are a base plus an offset, the waits for
+    //      K and V come before those for P, and a block's MMAs and commits are
+    //      issued in one go.  (A second issuer for the other tile was slower:
+    //      the pipe then interleaves the two tiles' products and finishes both
+    //      late; packed prompts of 12k tokens 1.48 -> 2.46 ms.) ----
     constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
     constexpr uint32_t ID_S = (1u << 4) | FMT | ((uint32_t)(VA_ROWS >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
-    int ring = 0, nseg = 0, np[2] = {0, 0};
+    // descriptors of Q tile 0 and of K and V in stage 0 (the offsets stay inside the address field)
+    const uint64_t q_desc = sdesc_sw128(smem_u32(sm)), k_desc = sdesc_sw128(smem_u32(sm) + G::OFF_KV);
+    const uint64_t v_desc = sdesc_mn_sw128(smem_u32(sm) + G::OFF_KV, VA_ROWS * 128);
+    int ring = 0, nseg = 0;
+    uint32_t np[2] = {0u, 0u};
     bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+      ok = ok && va_wait(bar, ph, abort_flag, P.err);
+      tc_fence_after();
+    };
     for (; ok && seg.next(P); ++nseg) {
-      const int n = seg.n, nbp = TREE ? va_blocks(seg.q.avail) : 0;
+      const int n = seg.n;
+      const uint64_t q1_desc = q_desc + (seg.dual ? (G::TILE >> 4) : 0);
       auto at_k = [&](int i) { return ring + (i ? 2 * i - 1 : 0); };
       auto at_v = [&](int i) { return ring + (i < n - 1 ? 2 * i + 2 : 2 * n - 1); };
-      auto wait = [&](uint64_t* bar, uint32_t ph) {
-        ok = ok && va_wait(bar, ph, abort_flag, P.err);
-        tc_fence_after();
-      };
       auto kv_wait = [&](int at) { wait(&kv_full[at % NS], (at / NS) & 1); };
-      auto kv_done = [&](int at) {
-        if (ok && va_elect()) mma_commit(&kv_empty[at % NS]);
+      auto issue_s = [&](auto tile, int st) {   // S_t = Q K^T, K in stage st
+        constexpr int t = decltype(tile)::value;
+        const uint64_t qd = t ? q1_desc : q_desc, kd = k_desc + st * (G::TILE >> 4);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t o = ((ks >> 2) * (VA_ROWS * 128) + (ks & 3) * 32) >> 4;
+          mma_ss(tbase + G::S0 + t * 128, qd + o, kd + o, ID_S, ks > 0);
+        }
+        mma_commit(&s_full[t]);
       };
-      auto mma_s = [&](int t, int i) {   // S_t = Q K(i)^T (K(i) has been waited for)
-        const uint64_t qd = sdesc_sw128(smem_u32(sm) + (seg.dual ? t : 0) * G::TILE);
-        const uint64_t kd = sdesc_sw128(smem_u32(sm) + G::OFF_KV + (at_k(i) % NS) * G::TILE);
+      // O_t += P_t V(i), then S_t of block j (-1: none, O_t is complete).  `free`:
+      // V(i) and K(j) have no other reader.
+      auto advance = [&](auto tile, int i, bool first, int j, bool free) {
+        constexpr int t = decltype(tile)::value;
+        const int sv = at_v(i) % NS, sk = j >= 0 ? at_k(j) % NS : 0;
+        const uint64_t vd = v_desc + sv * (G::TILE >> 4);
+        const uint32_t ph = np[t]++ & 1;
+        wait(&p_full[2 * t], ph);
         if (ok && va_elect()) {
 #pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t o = ((ks >> 2) * (VA_ROWS * 128) + (ks & 3) * 32) >> 4;
-            mma_ss(tbase + G::S0 + t * 128, qd + o, kd + o, ID_S, ks > 0);
+          for (int ks = 0; ks < 4; ++ks)
+            mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + ks * 8, vd + ks * (2048 >> 4), ID_O, !(first && ks == 0));
+        }
+        wait(&p_full[2 * t + 1], ph);
+        if (ok && va_elect()) {
+#pragma unroll
+          for (int ks = 4; ks < 8; ++ks)
+            mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + 64 + (ks & 3) * 8, vd + ks * (2048 >> 4), ID_O, 1u);
+          if (free) mma_commit(&kv_empty[sv]);
+          if (j >= 0) {
+            issue_s(tile, sk);
+            if (free) mma_commit(&kv_empty[sk]);
+            if (free && j == n - 1) mma_commit(q_empty);
+          } else {
+            mma_commit(&o_full[t]);
           }
-          mma_commit(&s_full[t]);
         }
       };
-      auto v_ready = [&](int i) {   // V(i) is there, and its rows past the sequence's keys are zero
-        kv_wait(at_v(i));
+      // Drafted nodes that any node's mask names, blocks 0 and 1 of the drafts
+      // (read while the first block's softmax runs).
+      const int nbp = TREE ? va_blocks(seg.q.avail) : 0;
+      uint32_t named[8];
+      auto read_named = [&] {
+        if (!TREE || seg.b0 + n <= nbp) return;
+        const int words = 2 * P.words;
+        const uint32_t* rows = P.mask + (size_t)seg.s * P.T * words;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) named[w] = 0u;
+        for (int r = lane; r < seg.q.n; r += 32) {
+#pragma unroll
+          for (int w = 0; w < 8; ++w)
+            if (w < words) named[w] |= rows[(size_t)r * words + w];
+        }
+#pragma unroll
+        for (int w = 0; w < 8; ++w) named[w] = __reduce_or_sync(0xffffffffu, named[w]);
+      };
+      // Rows of V(i) that no row of the item sees are cleared: their weights are
+      // 0, but 0 * (whatever lies there) may be NaN.
+      auto clear = [&](int i) {
         const int b = seg.b0 + i;
-        const int valid = TREE && b >= nbp ? seg.q.n - (b - nbp) * VA_ROWS : seg.q.avail - b * VA_ROWS;
-        if (ok && valid < VA_ROWS) {   // their weights are 0, but 0 * (whatever lies there) may be NaN
-          uint8_t* v = sm + G::OFF_KV + (at_v(i) % NS) * G::TILE;
-          for (int hf = 0; hf < HALVES; ++hf)
-            for (int o = max(0, valid) * 128 + lane * 16; o < VA_ROWS * 128; o += 512)
-              *reinterpret_cast<uint4*>(v + hf * (VA_ROWS * 128) + o) = make_uint4(0u, 0u, 0u, 0u);
+        const bool draft = TREE && b >= nbp;
+        const int valid = draft ? seg.q.n - (b - nbp) * VA_ROWS : seg.q.avail - b * VA_ROWS;
+        uint8_t* v = sm + G::OFF_KV + (at_v(i) % NS) * G::TILE + (lane & 7) * 16;
+        bool any = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t seen = va_bits_below(valid, w);
+          if (draft) seen &= b > nbp ? named[4 + w] : named[w];
+          if (seen == 0xffffffffu) continue;
+          any = true;
+          for (int r = lane >> 3; r < 32; r += 4)   // 8 lanes clear one row's 128 bytes
+            if (!(seen >> r & 1u))
+              for (int hf = 0; hf < HALVES; ++hf)
+                *reinterpret_cast<uint4*>(v + hf * (VA_ROWS * 128) + (w * 32 + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (any) {
           fence_proxy_async();
           __syncwarp();
         }
       };
-      auto mma_o = [&](int t, int i, bool first) {   // O_t += P_t V(i)
-        const uint64_t vd = sdesc_mn_sw128(smem_u32(sm) + G::OFF_KV + (at_v(i) % NS) * G::TILE, VA_ROWS * 128);
-        const uint32_t ph = np[t]++ & 1;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          wait(&p_full[2 * t + half], ph);
-          if (ok && va_elect()) {
-#pragma unroll
-            for (int ks = half * 4; ks < half * 4 + 4; ++ks)
-              mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + half * 64 + (ks & 3) * 8, vd + ks * (2048 >> 4), ID_O,
-                     !(first && ks == 0));
-          }
-        }
-      };
-      auto o_done = [&](int t) {
-        if (ok && va_elect()) mma_commit(&o_full[t]);
-      };
-      auto q_done = [&] {
-        if (ok && va_elect()) mma_commit(q_empty);
-      };
+      // the first block that is not whole: a prefix's or prompt's end, then the drafts
+      const int ragged = seg.q.avail / VA_ROWS - seg.b0;
+      constexpr std::integral_constant<int, 0> T0{};
+      constexpr std::integral_constant<int, 1> T1{};
       wait(q_full, nseg & 1);
       kv_wait(at_k(0));
       if (seg.dual) {
-        if (seg.n0 > 0) mma_s(0, 0);
-        mma_s(1, 0);
-        kv_done(at_k(0));
-        if (n == 1) q_done();
+        if (ok && va_elect()) {
+          const int st = at_k(0) % NS;
+          if (seg.n0 > 0) issue_s(T0, st);
+          issue_s(T1, st);
+          mma_commit(&kv_empty[st]);
+          if (n == 1) mma_commit(q_empty);
+        }
+        read_named();
         for (int i = 0; i < n && ok; ++i) {
-          v_ready(i);
-          if (i + 1 < n) kv_wait(at_k(i + 1));
-          if (i < seg.n0) {
-            mma_o(0, i, i == 0);
-            if (i + 1 < seg.n0) mma_s(0, i + 1);
-            else o_done(0);
-          }
-          mma_o(1, i, i == 0);
-          kv_done(at_v(i));
-          if (i + 1 < n) {
-            mma_s(1, i + 1);
-            kv_done(at_k(i + 1));
-            if (i + 1 == n - 1) q_done();
-          } else {
-            o_done(1);
-          }
+          kv_wait(at_v(i));
+          if (i >= ragged && ok) clear(i);
+          const int j = i + 1 < n ? i + 1 : -1;
+          if (j >= 0) kv_wait(at_k(j));
+          if (i < seg.n0) advance(T0, i, i == 0, j < seg.n0 ? j : -1, false);
+          advance(T1, i, i == 0, j, true);
         }
       } else {
-        for (int i = 0; i < 2 && i < n; ++i) {
-          kv_wait(at_k(i));
-          mma_s(i, i);
-          kv_done(at_k(i));
-        }
-        if (n <= 2) q_done();
-        for (int i = 0; i < n && ok; ++i) {
-          v_ready(i);
-          if (i + 2 < n) kv_wait(at_k(i + 2));
-          mma_o(i & 1, i, i < 2);
-          kv_done(at_v(i));
-          if (i + 2 < n) {
-            mma_s(i & 1, i + 2);
-            kv_done(at_k(i + 2));
-            if (i + 2 == n - 1) q_done();
-          } else {
-            o_done(i & 1);
+        if (n > 1) kv_wait(at_k(1));
+        if (ok && va_elect()) {
+          issue_s(T0, at_k(0) % NS);
+          mma_commit(&kv_empty[at_k(0) % NS]);
+          if (n > 1) {
+            issue_s(T1, at_k(1) % NS);
+            mma_commit(&kv_empty[at_k(1) % NS]);
           }
+          if (n <= 2) mma_commit(q_empty);
+        }
+        read_named();
+        for (int i = 0; i < n && ok; ++i) {
+          kv_wait(at_v(i));
+          if (i >= ragged && ok) clear(i);
+          const int j = i + 2 < n ? i + 2 : -1;
+          if (j >= 0) kv_wait(at_k(j));
+          if (i & 1) advance(T1, i, i < 2, j, true);
+          else advance(T0, i, i < 2, j, true);
         }
       }
       ring += 2 * n;
