@@ -6,10 +6,12 @@ Public surface:
   (``W4A16GEMV``, the ``W4A16GEMM`` family, ``RMSNormRoPE``,
   ``LlamaChunkedAttention``, ``ResidualAddRMSNorm``, ``SiLUMul``,
   ``CopyPresentPacketKV``) backed by
-  CUDA kernels through the C-ABI library ``libt2b.so``;
+  CUDA kernels through the C-ABI library ``libt2b.so``, and the serving
+  operators (``PackedAttention``, ``DraftTreeAttention``, ``DraftTreeCommit``,
+  ``TokenLogProbs``);
 * ``torch2iron_b200.engine`` -- ``DecodeEngine``: the fused decode step (five
-  launches per layer, CUDA graph, programmatic dependent launch), chunked
-  prefill and greedy generation;
+  launches per layer, CUDA graph, programmatic dependent launch), chunked and
+  packed prefill, prompt scores, greedy generation and draft-tree decoding;
 * ``torch2iron_b200.tp`` -- ``TPDecodeEngine``: the same step tensor-parallel
   over NCCL ranks;
 * ``torch2iron_b200.loaders`` -- the reference's packed artifact and AutoGPTQ

