@@ -486,7 +486,9 @@ T2B_API int t2b_tree_attention(const void* q, const void* k_cache, const void* v
  * n_accepted[b].  A row with n_nodes[b] <= 0 or ctx_len[b] outside
  * [0, max_ctx) accepts nothing (next_token -1, new_len = ctx_len).  Every
  * other cache row stays as it is.  k_draft .. v_cache are HOST arrays of
- * n_layers device pointers; drafts and caches must not overlap.
+ * n_layers device pointers; drafts and caches must not overlap.  The results
+ * (path .. new_len) must not overlap the inputs nor one another (new_len is not
+ * ctx_len: T2B_ERR_ARG).
  */
 T2B_API int t2b_tree_commit(const int32_t* tokens, const int32_t* parents, const int32_t* predicted,
                             const int32_t* ctx_len, const int32_t* n_nodes, const void* const* k_draft,

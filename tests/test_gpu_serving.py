@@ -512,6 +512,15 @@ def test_commit_graph_replay():
                 assert torch.equal(kc[:, b, :, c + i], kd[:, b, n]) and torch.equal(vc[:, b, :, c + i], kd[:, b, n])
 
 
+def test_commit_in_place_is_refused():
+    z = lambda *s, dtype=BF: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    ctx, row = z(2, dtype=I32), lambda: z(2, dtype=I32)  # noqa: E731
+    op = DraftTreeCommit(layers=1, batch=2, nodes=3, max_ctx=64, num_kv_groups=2)
+    tree = [z(2, 3, dtype=I32) for _ in range(4)]
+    with pytest.raises(RuntimeError, match="argument"):
+        op(*tree[:3], ctx, z(1, 2, 3, 2, 64), z(1, 2, 3, 2, 64), z(1, 2, 2, 64, 64), z(1, 2, 2, 64, 64), tree[3], row(), row(), ctx)
+
+
 def test_commit_refusals_on_the_device():
     z = lambda *s, dtype=BF: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
     op = DraftTreeCommit(layers=2, batch=2, nodes=3, max_ctx=64, num_kv_groups=2)

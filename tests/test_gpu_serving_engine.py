@@ -193,6 +193,29 @@ def test_decode_tree_of_one_node_is_a_decode_step():
             assert max_abs(a.k_cache[li][r, :, :n + 1], b.k_cache[li][r, :, :n + 1]) <= 5e-2
 
 
+def test_serving_paths_between_captured_steps():
+    """Packed prefill, captured one-token steps and draft trees share the engine's state in any order."""
+    cfg, model = SMALL, synth.random_model(SMALL, seed=101)
+    prompts = ragged(cfg, [6, 25, 40], 102)
+    states = []
+    for graph in (False, True):
+        eng = DecodeEngine(cfg, model, batch=3, max_ctx=128, use_graph=graph)
+        eng.prefill_packed(prompts)
+        log = [eng.next_tokens.tolist()]
+        for _ in range(2):
+            eng.advance()
+            log.append(eng.next_tokens.tolist())
+            tok = np.stack([eng.tokens.cpu().numpy(), np.full(3, 7), np.full(3, 9)], 1)
+            log += [t.tolist() for t in eng.decode_tree(tok, np.tile([-1, 0, 0], (3, 1)))]
+        eng.prefill_packed(prompts, score=True)               # and again over the same caches
+        log.append(eng.next_tokens.tolist())
+        eng.advance()
+        log.append(eng.pos.tolist())
+        states.append(log)
+        eng.release()
+    assert states[0] == states[1] and states[0][0] == states[0][-2]
+
+
 def test_decode_tree_dead_and_full_rows_stay():
     cfg, model = SMALL, synth.random_model(SMALL, seed=91)
     eng = engine(cfg, model, 3, max_ctx=64)
@@ -206,6 +229,23 @@ def test_decode_tree_dead_and_full_rows_stay():
     assert following[:2].tolist() == [-1, -1] and path[:2].eq(-1).all()
     for a, b in zip(eng.k_cache, caches):
         assert torch.equal(a[:2], b[:2]) and torch.equal(a[2, :, :63], b[2, :, :63])
+
+
+def test_decode_tree_takes_padded_trees():
+    """Nodes behind num_nodes may hold any token and parent; a row's result does not depend on them."""
+    cfg, model = SMALL, synth.random_model(SMALL, seed=93)
+    prompts = ragged(cfg, [12, 30], 94)
+    got = []
+    for fill, T in ((-1, 6), (10 ** 6, 9)):
+        eng = engine(cfg, model, 2)
+        eng.prefill_packed(prompts)
+        tok, par = np.full((2, T), fill), np.full((2, T), fill)
+        tok[:, 0], par[:, 0] = eng.tokens.cpu().numpy(), -1
+        tok[0, 1:3], par[0, 1:3] = [3, 4], [0, 1]
+        path, count, following = eng.decode_tree(tok, par, num_nodes=torch.tensor([3, 1]))
+        assert (path[0] < 3).all() and (path[1] < 1).all()
+        got.append((count.tolist(), following.tolist(), eng.pos.tolist()))
+    assert got[0] == got[1]
 
 
 def test_packed_prefill_and_tree_refusals():

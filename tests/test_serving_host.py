@@ -193,6 +193,22 @@ def test_tree_commit_rejects_bad_arguments_on_the_host(base):
     assert call(kd_row=4) == ERR_ALIGN
 
 
+def test_tree_commit_refuses_results_over_inputs(base):
+    """Every CTA reads a row's inputs while one writes its results: an update in place would race."""
+    f = _lib.load().t2b_tree_commit
+    good = (C.c_void_p * 1)(base + 8192)
+
+    def call(ctx=base + 512, path=base + 1024, count=base + 1536, nxt=base + 2048, length=base + 2560, live=None):
+        return f(base, base + 128, base + 256, ctx, live, good, good, good, good, 1, path, count, nxt, length, 2, 4, 2, 64,
+                 64, 512, 128, 64, 512, 128, 64, None)
+
+    assert call(length=base + 512) == ERR_ARG                  # new_len over ctx_len
+    assert call(path=base + 124) == ERR_ARG                    # path over tokens and parents
+    assert call(nxt=base + 1540) == ERR_ARG                    # next_token over num_accepted
+    assert call(live=base + 2560) == ERR_ARG                   # new_len over num_nodes
+    assert call(count=base + 256) == ERR_ARG
+
+
 def test_token_logprobs_rejects_bad_arguments_on_the_host(base):
     f = _lib.load().t2b_token_logprobs
 

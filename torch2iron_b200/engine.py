@@ -729,11 +729,15 @@ class DecodeEngine:
         par = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
         if tok.ndim != 2 or tok.shape[0] != B or tok.shape != par.shape or not 1 <= tok.shape[1] <= 256:
             raise ValueError(f"decode_tree takes tokens and parents [{B}, nodes] with nodes in 1..256")
-        if not np.issubdtype(tok.dtype, np.integer) or tok.min() < 0 or tok.max() >= cfg.vocab_size:
-            raise ValueError(f"token ids must be integers in [0, {cfg.vocab_size})")
         T = tok.shape[1]
+        if isinstance(num_nodes, torch.Tensor):
+            num_nodes = num_nodes.cpu().numpy()
         mask, depth = draft_tree(par, num_nodes)
         live = np.full(B, T) if num_nodes is None else np.asarray(num_nodes).reshape(-1)
+        used = np.arange(T)[None] < live[:, None]
+        if not np.issubdtype(tok.dtype, np.integer) or ((tok < 0) | (tok >= cfg.vocab_size))[used].any():
+            raise ValueError(f"token ids must be integers in [0, {cfg.vocab_size})")
+        tok = np.where(used, tok, 0)                      # (padding may hold anything)
         M, tb, pf = B * T, self._tree_buffers(T), self._prefill_buffers(B * T)
         tb["tree"].copy_(torch.from_numpy(np.stack([tok, par, depth.numpy()]).astype(np.int32)))
         tb["live"].copy_(torch.from_numpy(live.astype(np.int32)))

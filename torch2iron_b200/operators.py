@@ -705,8 +705,9 @@ class DraftTreeCommit:
     are ``[layers, batch, nodes, kv, head_dim]`` or a sequence of one tensor per
     layer, ``k_caches`` / ``v_caches`` likewise ``[layers, batch, kv, max_ctx,
     head_dim]``.  Writes ``path`` (-1 behind the walk's end), ``num_accepted``,
-    ``next_token`` and ``new_len = ctx_len + num_accepted``; a row with no live
-    node or no room accepts nothing (next token -1)."""
+    ``next_token`` and ``new_len = ctx_len + num_accepted``, none of them one of
+    the inputs; a row with no live node or no room accepts nothing (next token
+    -1)."""
 
     layers: int
     batch: int
