@@ -168,6 +168,24 @@ def test_packed_strided_views():
     assert torch.equal(other, out)
 
 
+@pytest.mark.parametrize("heads", [(4, 2, 64), (6, 2, 128), (5, 1, 64)])
+def test_packed_results_do_not_depend_on_rows_outside(heads):
+    """The same bits whatever lies in the rows before, between and behind the sequences' own."""
+    nh, nkv, hd = heads
+    g, n = gen(50), [700, 30, 260]
+    total = sum(n) + 40
+    q, k, v = randn(g, total, nh, hd, scale=4.0), randn(g, total, nkv, hd), randn(g, total, nkv, hd)
+    op = PackedAttention(tokens=total, num_seqs=3, num_kv_groups=nkv, q_heads_per_group=nh // nkv, head_dim=hd)
+    start, got = ints([0, 700, 730, 990]), []
+    for fill in (0.0, 300.0, -math.inf, math.nan):
+        q[990:] = fill
+        out, lse = torch.empty_like(q), torch.empty(total, nh, device="cuda")
+        op(q, k, v, start, out, lse=lse)
+        got.append((out[:990].clone(), lse[:990].clone()))
+    for out, lse in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(lse, got[0][1])
+
+
 def test_packed_refusals_on_the_device():
     op = PackedAttention(tokens=4, num_seqs=1, num_kv_groups=2, q_heads_per_group=2, head_dim=64)
     q, kv, start = torch.zeros(4, 4, 64, dtype=BF, device="cuda"), torch.zeros(4, 2, 64, dtype=BF, device="cuda"), ints([0, 4])
@@ -321,6 +339,13 @@ def test_tree_heads_and_types(heads, dtype):
 
 def test_tree_ragged_batch_with_dead_rows():
     check_tree(6, 20, [300, 0, 64, 5, 1, 130], (8, 2, 128), live=[20, 3, 0, 1, 19, 7])
+
+
+def test_tree_with_rows_left_over_in_a_tile_repeats_its_bits():
+    """3 q heads per kv head leave 2 of a tile's 128 rows unused: what lies there decides nothing."""
+    for seed in range(3):
+        check_tree(3, 129, [2602, 256, 256], (24, 8, 128), live=[118, 82, 124], seed=seed)
+    check_tree(2, 40, [1500, 900], (5, 1, 64))
 
 
 def test_tree_rows_that_see_nothing():

@@ -834,8 +834,9 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
         if (!ok) s_bad[pair] = 1;
-        // (behind this barrier both halves hold their scores: P may go over S)
-        if (va_pair_any(bar, top > m + VA_ROOM || !ok)) {
+        // (behind this barrier both halves hold their scores; a row that is not live
+        // holds whatever was there, and must not decide when its neighbours rescale)
+        if (va_pair_any(bar, (live && top > m + VA_ROOM) || !ok)) {
           if (u) *x_slot = top;
           va_pair_sync(bar);
           if (s_bad[pair]) {
