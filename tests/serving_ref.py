@@ -16,10 +16,17 @@ def attention_rows(q, k, v, seen, scale):
     in 32 bits and rounds each softmax weight once to the operands' type:
     a score is off by at most (hd + 2) 2^-24 sum |q k| scale, a weight by twice
     that (its own exponential and the sum it is divided by) plus half a step
-    of its type, and the result is rounded once more (``out_tolerance``)."""
+    of its type, and the result is rounded once more (``assert_attention``).
+
+    fp16 has a least normal number, 2^-14, below which its half step is 2^-25
+    and no longer relative.  The kernels scale the weights so that a row's
+    largest is at least 2^7 (its exponent's reference is never less than 7
+    under the running maximum), so the sum that divides them is at least 2^7
+    too, and a small weight adds at most 2^-25 / 2^7 |v| = 2^-32 |v|."""
     n, nh, hd = q.shape
     nkv = k.shape[1]
     u = torch.finfo(q.dtype).eps / 2
+    least = 2.0 ** -32 if q.dtype == torch.float16 else 0.0
     q, k, v = (t.double().cpu() for t in (q, k, v))
     seen = seen.cpu()
     out = torch.zeros(n, nh, hd, dtype=torch.float64)
@@ -39,17 +46,17 @@ def attention_rows(q, k, v, seen, scale):
         off = ((q[:, h].abs() @ kh.abs().t() * scale).masked_fill(~seen, 0.0).amax(1) * (hd + 2) * 2.0 ** -24
                + LOG2E_ULP)
         terms = seen.sum(1).clamp(min=1).double().log2() + 130       # additions a partial sum goes through
-        err[:, h] = (u + 2 * off + terms * 2.0 ** -24)[:, None] * (p @ vh.abs())
+        err[:, h] = (u + 2 * off + terms * 2.0 ** -24)[:, None] * (p @ vh.abs()) + least * (seen.double() @ vh.abs())
         lse_err[:, h] = off + terms * 2.0 ** -24 + torch.where(live, lse[:, h].abs(), 0.0) * 2.0 ** -22
     return out, lse, err, lse_err
 
 
 def assert_attention(out, lse, want):
     ref, ref_lse, err, lse_err = want
-    u = torch.finfo(out.dtype).eps / 2
+    u, tiny = torch.finfo(out.dtype).eps / 2, torch.finfo(out.dtype).tiny     # below tiny a half step is u * tiny
     got = out.double().cpu()
     assert torch.isfinite(got).all()
-    tol = err + u * (ref.abs() + err) + 2.0 ** -30
+    tol = err + u * (ref.abs() + err).clamp(min=tiny) + 2.0 ** -30
     worst = ((got - ref).abs() / tol).max()
     assert worst <= 1, f"output off by {float(worst):.3g} of its bound"
     if lse is not None:
