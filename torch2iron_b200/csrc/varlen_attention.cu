@@ -555,216 +555,216 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
 
   const int tpt = P.tpt, qpg = P.qpg;
   if (warp >= VA_WARP_TMA) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(VA_REGS_OTHER));
-  VaWalk<TREE> seg(start, units);
-  if (warp == VA_WARP_TMA) {
-    // ---- TMA: per segment K0, (Q), K1, V0, K2, V1, ..: the order the MMAs take them ----
-    if (lane == 0) {
-      int pos = 0, nseg = 0, q_loads = 0;
-      bool ok = true;
-      int4 tail = make_int4(0, 0, 0, 0), first = make_int4(0, 0, 0, 0);   // this CTA's ends, for the joining kernel
-      for (; ok && seg.next(P); ++nseg) {
-        if (nseg == 0) first = make_int4(seg.b0 > 0, seg.b0 + seg.n == seg.nb, 0, 0);
-        if (seg.b0 == 0 && seg.n < seg.nb) tail = make_int4(seg.s, seg.p, seg.g, 1);
-        auto load_q = [&] {
-          if (nseg > 0) ok = mbar_wait_bounded(q_empty, (nseg - 1) & 1, P.err);
-          if (!ok) return;
-          const int tiles = seg.dual ? 2 : 1, row = seg.q.q0 + 2 * seg.p * tpt;
-          mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * HALVES * tpt * qpg * 128));
-          for (int t = 0; t < tiles; ++t)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(VA_REGS_OTHER));
+    VaWalk<TREE> seg(start, units);
+    if (warp == VA_WARP_TMA) {
+      // ---- TMA: per segment K0, (Q), K1, V0, K2, V1, ..: the order the MMAs take them ----
+      if (lane == 0) {
+        int pos = 0, nseg = 0, q_loads = 0;
+        bool ok = true;
+        int4 tail = make_int4(0, 0, 0, 0), first = make_int4(0, 0, 0, 0);   // this CTA's ends, for the joining kernel
+        for (; ok && seg.next(P); ++nseg) {
+          if (nseg == 0) first = make_int4(seg.b0 > 0, seg.b0 + seg.n == seg.nb, 0, 0);
+          if (seg.b0 == 0 && seg.n < seg.nb) tail = make_int4(seg.s, seg.p, seg.g, 1);
+          auto load_q = [&] {
+            if (nseg > 0) ok = mbar_wait_bounded(q_empty, (nseg - 1) & 1, P.err);
+            if (!ok) return;
+            const int tiles = seg.dual ? 2 : 1, row = seg.q.q0 + 2 * seg.p * tpt;
+            mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * HALVES * tpt * qpg * 128));
+            for (int t = 0; t < tiles; ++t)
+              for (int hf = 0; hf < HALVES; ++hf)
+                tma_load_3d(sm + t * G::TILE + hf * (VA_ROWS * 128), &P.qmap, hf * 64, seg.g * qpg, row + t * tpt, q_full);
+            q_loads = nseg + 1;
+          };
+          if (nseg == 0) load_q();
+          const int nbp = TREE ? va_blocks(seg.q.avail) : 0;
+          const int seq = TREE || P.cached ? seg.s : 0;
+          for (int i = 0; ok && i < 2 * seg.n; ++i, ++pos) {
+            const bool is_k = i == 0 || ((i & 1) && i < 2 * seg.n - 1);
+            const int b = seg.b0 + (is_k ? (i + 1) / 2 : i == 2 * seg.n - 1 ? seg.n - 1 : i / 2 - 1);
+            const int st = pos % NS;
+            if (pos >= NS) ok = mbar_wait_bounded(&kv_empty[st], ((pos / NS) - 1) & 1, P.err);
+            if (!ok || *abort_flag) {
+              ok = false;
+              break;
+            }
+            const bool draft = TREE && b >= nbp;
+            const void* map = draft ? (is_k ? &P.kdmap : &P.vdmap) : (is_k ? &P.kmap : &P.vmap);
+            const int tok = draft ? (b - nbp) * VA_ROWS : seg.q.first + b * VA_ROWS;
+            uint8_t* dst = sm + G::OFF_KV + st * G::TILE;
+            mbar_arrive_expect_tx(&kv_full[st], (uint32_t)G::TILE);
             for (int hf = 0; hf < HALVES; ++hf)
-              tma_load_3d(sm + t * G::TILE + hf * (VA_ROWS * 128), &P.qmap, hf * 64, seg.g * qpg, row + t * tpt, q_full);
-          q_loads = nseg + 1;
-        };
-        if (nseg == 0) load_q();
-        const int nbp = TREE ? va_blocks(seg.q.avail) : 0;
-        const int seq = TREE || P.cached ? seg.s : 0;
-        for (int i = 0; ok && i < 2 * seg.n; ++i, ++pos) {
-          const bool is_k = i == 0 || ((i & 1) && i < 2 * seg.n - 1);
-          const int b = seg.b0 + (is_k ? (i + 1) / 2 : i == 2 * seg.n - 1 ? seg.n - 1 : i / 2 - 1);
-          const int st = pos % NS;
-          if (pos >= NS) ok = mbar_wait_bounded(&kv_empty[st], ((pos / NS) - 1) & 1, P.err);
-          if (!ok || *abort_flag) {
-            ok = false;
-            break;
+              tma_load_4d(dst + hf * (VA_ROWS * 128), map, hf * 64, tok, seg.g, seq, &kv_full[st]);
+            if (i == 1 && nseg > 0) load_q();
           }
-          const bool draft = TREE && b >= nbp;
-          const void* map = draft ? (is_k ? &P.kdmap : &P.vdmap) : (is_k ? &P.kmap : &P.vmap);
-          const int tok = draft ? (b - nbp) * VA_ROWS : seg.q.first + b * VA_ROWS;
-          uint8_t* dst = sm + G::OFF_KV + st * G::TILE;
-          mbar_arrive_expect_tx(&kv_full[st], (uint32_t)G::TILE);
-          for (int hf = 0; hf < HALVES; ++hf)
-            tma_load_4d(dst + hf * (VA_ROWS * 128), map, hf * 64, tok, seg.g, seq, &kv_full[st]);
-          if (i == 1 && nseg > 0) load_q();
         }
+        if (!ok) *abort_flag = 1;
+        // every load has landed before the CTA may exit
+        for (int i = max(0, pos - NS); i < pos; ++i) mbar_wait_bounded(&kv_full[i % NS], (i / NS) & 1, P.err);
+        if (q_loads) mbar_wait_bounded(q_full, (q_loads - 1) & 1, P.err);
+        if (!ok) tail.w = first.x = 0;
+        P.head[2 * c] = tail;
+        P.head[2 * c + 1] = first;
+      }
+    } else if (warp == VA_WARP_MMA) {
+      // ---- MMA issuer (one lane; the others help to clear V rows).  It shares its
+      //      scheduler with four softmax warps, so every instruction here delays
+      //      the tensor pipe: descriptors are a base plus an offset, the waits for
+      //      K and V come before those for P, and a block's MMAs and commits are
+      //      issued in one go.  (A second issuer for the other tile was slower:
+      //      the pipe then interleaves the two tiles' products and finishes both
+      //      late; packed prompts of 12k tokens 1.48 -> 2.46 ms.) ----
+      constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
+      constexpr uint32_t ID_S = (1u << 4) | FMT | ((uint32_t)(VA_ROWS >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
+      constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
+      // descriptors of Q tile 0 and of K and V in stage 0 (the offsets stay inside the address field)
+      const uint64_t q_desc = sdesc_sw128(smem_u32(sm)), k_desc = sdesc_sw128(smem_u32(sm) + G::OFF_KV);
+      const uint64_t v_desc = sdesc_mn_sw128(smem_u32(sm) + G::OFF_KV, VA_ROWS * 128);
+      int ring = 0, nseg = 0;
+      uint32_t np[2] = {0u, 0u};
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t ph) {
+        ok = ok && va_wait(bar, ph, abort_flag, P.err);
+        tc_fence_after();
+      };
+      for (; ok && seg.next(P); ++nseg) {
+        const int n = seg.n;
+        const uint64_t q1_desc = q_desc + (seg.dual ? (G::TILE >> 4) : 0);
+        auto at_k = [&](int i) { return ring + (i ? 2 * i - 1 : 0); };
+        auto at_v = [&](int i) { return ring + (i < n - 1 ? 2 * i + 2 : 2 * n - 1); };
+        auto kv_wait = [&](int at) { wait(&kv_full[at % NS], (at / NS) & 1); };
+        auto issue_s = [&](auto tile, int st) {   // S_t = Q K^T, K in stage st
+          constexpr int t = decltype(tile)::value;
+          const uint64_t qd = t ? q1_desc : q_desc, kd = k_desc + st * (G::TILE >> 4);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t o = ((ks >> 2) * (VA_ROWS * 128) + (ks & 3) * 32) >> 4;
+            mma_ss(tbase + G::S0 + t * 128, qd + o, kd + o, ID_S, ks > 0);
+          }
+          mma_commit(&s_full[t]);
+        };
+        // O_t += P_t V(i), then S_t of block j (-1: none, O_t is complete).  `free`:
+        // V(i) and K(j) have no other reader.
+        auto advance = [&](auto tile, int i, bool first, int j, bool free) {
+          constexpr int t = decltype(tile)::value;
+          const int sv = at_v(i) % NS, sk = j >= 0 ? at_k(j) % NS : 0;
+          const uint64_t vd = v_desc + sv * (G::TILE >> 4);
+          const uint32_t ph = np[t]++ & 1;
+          wait(&p_full[2 * t], ph);
+          if (ok && va_elect()) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + ks * 8, vd + ks * (2048 >> 4), ID_O, !(first && ks == 0));
+          }
+          wait(&p_full[2 * t + 1], ph);
+          if (ok && va_elect()) {
+#pragma unroll
+            for (int ks = 4; ks < 8; ++ks)
+              mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + 64 + (ks & 3) * 8, vd + ks * (2048 >> 4), ID_O, 1u);
+            if (free) mma_commit(&kv_empty[sv]);
+            if (j >= 0) {
+              issue_s(tile, sk);
+              if (free) mma_commit(&kv_empty[sk]);
+              if (free && j == n - 1) mma_commit(q_empty);
+            } else {
+              mma_commit(&o_full[t]);
+            }
+          }
+        };
+        // Drafted nodes that any node's mask names, blocks 0 and 1 of the drafts
+        // (read while the first block's softmax runs).
+        const int nbp = TREE ? va_blocks(seg.q.avail) : 0;
+        uint32_t named[8];
+        auto read_named = [&] {
+          if (!TREE || seg.b0 + n <= nbp) return;
+          const int words = 2 * P.words;
+          const uint32_t* rows = P.mask + (size_t)seg.s * P.T * words;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) named[w] = 0u;
+          for (int r = lane; r < seg.q.n; r += 32) {
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+              if (w < words) named[w] |= rows[(size_t)r * words + w];
+          }
+#pragma unroll
+          for (int w = 0; w < 8; ++w) named[w] = __reduce_or_sync(0xffffffffu, named[w]);
+        };
+        // Rows of V(i) that no row of the item sees are cleared: their weights are
+        // 0, but 0 * (whatever lies there) may be NaN.
+        auto clear = [&](int i) {
+          const int b = seg.b0 + i;
+          const bool draft = TREE && b >= nbp;
+          const int valid = draft ? seg.q.n - (b - nbp) * VA_ROWS : seg.q.avail - b * VA_ROWS;
+          uint8_t* v = sm + G::OFF_KV + (at_v(i) % NS) * G::TILE + (lane & 7) * 16;
+          bool any = false;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t seen = va_bits_below(valid, w);
+            if (draft) seen &= b > nbp ? named[4 + w] : named[w];
+            if (seen == 0xffffffffu) continue;
+            any = true;
+            for (int r = lane >> 3; r < 32; r += 4)   // 8 lanes clear one row's 128 bytes
+              if (!(seen >> r & 1u))
+                for (int hf = 0; hf < HALVES; ++hf)
+                  *reinterpret_cast<uint4*>(v + hf * (VA_ROWS * 128) + (w * 32 + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          if (any) {
+            fence_proxy_async();
+            __syncwarp();
+          }
+        };
+        // the first block that is not whole: a prefix's or prompt's end, then the drafts
+        const int ragged = seg.q.avail / VA_ROWS - seg.b0;
+        constexpr std::integral_constant<int, 0> T0{};
+        constexpr std::integral_constant<int, 1> T1{};
+        wait(q_full, nseg & 1);
+        kv_wait(at_k(0));
+        if (seg.dual) {
+          if (ok && va_elect()) {
+            const int st = at_k(0) % NS;
+            if (seg.n0 > 0) issue_s(T0, st);
+            issue_s(T1, st);
+            mma_commit(&kv_empty[st]);
+            if (n == 1) mma_commit(q_empty);
+          }
+          read_named();
+          for (int i = 0; i < n && ok; ++i) {
+            kv_wait(at_v(i));
+            if (i >= ragged && ok) clear(i);
+            const int j = i + 1 < n ? i + 1 : -1;
+            if (j >= 0) kv_wait(at_k(j));
+            if (i < seg.n0) advance(T0, i, i == 0, j < seg.n0 ? j : -1, false);
+            advance(T1, i, i == 0, j, true);
+          }
+        } else {
+          if (n > 1) kv_wait(at_k(1));
+          if (ok && va_elect()) {
+            issue_s(T0, at_k(0) % NS);
+            mma_commit(&kv_empty[at_k(0) % NS]);
+            if (n > 1) {
+              issue_s(T1, at_k(1) % NS);
+              mma_commit(&kv_empty[at_k(1) % NS]);
+            }
+            if (n <= 2) mma_commit(q_empty);
+          }
+          read_named();
+          for (int i = 0; i < n && ok; ++i) {
+            kv_wait(at_v(i));
+            if (i >= ragged && ok) clear(i);
+            const int j = i + 2 < n ? i + 2 : -1;
+            if (j >= 0) kv_wait(at_k(j));
+            if (i & 1) advance(T1, i, i < 2, j, true);
+            else advance(T0, i, i < 2, j, true);
+          }
+        }
+        ring += 2 * n;
       }
       if (!ok) *abort_flag = 1;
-      // every load has landed before the CTA may exit
-      for (int i = max(0, pos - NS); i < pos; ++i) mbar_wait_bounded(&kv_full[i % NS], (i / NS) & 1, P.err);
-      if (q_loads) mbar_wait_bounded(q_full, (q_loads - 1) & 1, P.err);
-      if (!ok) tail.w = first.x = 0;
-      P.head[2 * c] = tail;
-      P.head[2 * c + 1] = first;
+      // every MMA issued here has retired before TMEM is released
+      __syncwarp();
+      if (va_elect()) mma_commit(done);
+      mbar_wait_bounded(done, 0, P.err);
     }
-  } else if (warp == VA_WARP_MMA) {
-    // ---- MMA issuer (one lane; the others help to clear V rows).  It shares its
-    //      scheduler with four softmax warps, so every instruction here delays
-    //      the tensor pipe: descriptors are a base plus an offset, the waits for
-    //      K and V come before those for P, and a block's MMAs and commits are
-    //      issued in one go.  (A second issuer for the other tile was slower:
-    //      the pipe then interleaves the two tiles' products and finishes both
-    //      late; packed prompts of 12k tokens 1.48 -> 2.46 ms.) ----
-    constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
-    constexpr uint32_t ID_S = (1u << 4) | FMT | ((uint32_t)(VA_ROWS >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
-    constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(VA_ROWS >> 4) << 24);
-    // descriptors of Q tile 0 and of K and V in stage 0 (the offsets stay inside the address field)
-    const uint64_t q_desc = sdesc_sw128(smem_u32(sm)), k_desc = sdesc_sw128(smem_u32(sm) + G::OFF_KV);
-    const uint64_t v_desc = sdesc_mn_sw128(smem_u32(sm) + G::OFF_KV, VA_ROWS * 128);
-    int ring = 0, nseg = 0;
-    uint32_t np[2] = {0u, 0u};
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t ph) {
-      ok = ok && va_wait(bar, ph, abort_flag, P.err);
-      tc_fence_after();
-    };
-    for (; ok && seg.next(P); ++nseg) {
-      const int n = seg.n;
-      const uint64_t q1_desc = q_desc + (seg.dual ? (G::TILE >> 4) : 0);
-      auto at_k = [&](int i) { return ring + (i ? 2 * i - 1 : 0); };
-      auto at_v = [&](int i) { return ring + (i < n - 1 ? 2 * i + 2 : 2 * n - 1); };
-      auto kv_wait = [&](int at) { wait(&kv_full[at % NS], (at / NS) & 1); };
-      auto issue_s = [&](auto tile, int st) {   // S_t = Q K^T, K in stage st
-        constexpr int t = decltype(tile)::value;
-        const uint64_t qd = t ? q1_desc : q_desc, kd = k_desc + st * (G::TILE >> 4);
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t o = ((ks >> 2) * (VA_ROWS * 128) + (ks & 3) * 32) >> 4;
-          mma_ss(tbase + G::S0 + t * 128, qd + o, kd + o, ID_S, ks > 0);
-        }
-        mma_commit(&s_full[t]);
-      };
-      // O_t += P_t V(i), then S_t of block j (-1: none, O_t is complete).  `free`:
-      // V(i) and K(j) have no other reader.
-      auto advance = [&](auto tile, int i, bool first, int j, bool free) {
-        constexpr int t = decltype(tile)::value;
-        const int sv = at_v(i) % NS, sk = j >= 0 ? at_k(j) % NS : 0;
-        const uint64_t vd = v_desc + sv * (G::TILE >> 4);
-        const uint32_t ph = np[t]++ & 1;
-        wait(&p_full[2 * t], ph);
-        if (ok && va_elect()) {
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + ks * 8, vd + ks * (2048 >> 4), ID_O, !(first && ks == 0));
-        }
-        wait(&p_full[2 * t + 1], ph);
-        if (ok && va_elect()) {
-#pragma unroll
-          for (int ks = 4; ks < 8; ++ks)
-            mma_ts(tbase + G::O0 + t * HD, tbase + G::S0 + t * 128 + 64 + (ks & 3) * 8, vd + ks * (2048 >> 4), ID_O, 1u);
-          if (free) mma_commit(&kv_empty[sv]);
-          if (j >= 0) {
-            issue_s(tile, sk);
-            if (free) mma_commit(&kv_empty[sk]);
-            if (free && j == n - 1) mma_commit(q_empty);
-          } else {
-            mma_commit(&o_full[t]);
-          }
-        }
-      };
-      // Drafted nodes that any node's mask names, blocks 0 and 1 of the drafts
-      // (read while the first block's softmax runs).
-      const int nbp = TREE ? va_blocks(seg.q.avail) : 0;
-      uint32_t named[8];
-      auto read_named = [&] {
-        if (!TREE || seg.b0 + n <= nbp) return;
-        const int words = 2 * P.words;
-        const uint32_t* rows = P.mask + (size_t)seg.s * P.T * words;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) named[w] = 0u;
-        for (int r = lane; r < seg.q.n; r += 32) {
-#pragma unroll
-          for (int w = 0; w < 8; ++w)
-            if (w < words) named[w] |= rows[(size_t)r * words + w];
-        }
-#pragma unroll
-        for (int w = 0; w < 8; ++w) named[w] = __reduce_or_sync(0xffffffffu, named[w]);
-      };
-      // Rows of V(i) that no row of the item sees are cleared: their weights are
-      // 0, but 0 * (whatever lies there) may be NaN.
-      auto clear = [&](int i) {
-        const int b = seg.b0 + i;
-        const bool draft = TREE && b >= nbp;
-        const int valid = draft ? seg.q.n - (b - nbp) * VA_ROWS : seg.q.avail - b * VA_ROWS;
-        uint8_t* v = sm + G::OFF_KV + (at_v(i) % NS) * G::TILE + (lane & 7) * 16;
-        bool any = false;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t seen = va_bits_below(valid, w);
-          if (draft) seen &= b > nbp ? named[4 + w] : named[w];
-          if (seen == 0xffffffffu) continue;
-          any = true;
-          for (int r = lane >> 3; r < 32; r += 4)   // 8 lanes clear one row's 128 bytes
-            if (!(seen >> r & 1u))
-              for (int hf = 0; hf < HALVES; ++hf)
-                *reinterpret_cast<uint4*>(v + hf * (VA_ROWS * 128) + (w * 32 + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        if (any) {
-          fence_proxy_async();
-          __syncwarp();
-        }
-      };
-      // the first block that is not whole: a prefix's or prompt's end, then the drafts
-      const int ragged = seg.q.avail / VA_ROWS - seg.b0;
-      constexpr std::integral_constant<int, 0> T0{};
-      constexpr std::integral_constant<int, 1> T1{};
-      wait(q_full, nseg & 1);
-      kv_wait(at_k(0));
-      if (seg.dual) {
-        if (ok && va_elect()) {
-          const int st = at_k(0) % NS;
-          if (seg.n0 > 0) issue_s(T0, st);
-          issue_s(T1, st);
-          mma_commit(&kv_empty[st]);
-          if (n == 1) mma_commit(q_empty);
-        }
-        read_named();
-        for (int i = 0; i < n && ok; ++i) {
-          kv_wait(at_v(i));
-          if (i >= ragged && ok) clear(i);
-          const int j = i + 1 < n ? i + 1 : -1;
-          if (j >= 0) kv_wait(at_k(j));
-          if (i < seg.n0) advance(T0, i, i == 0, j < seg.n0 ? j : -1, false);
-          advance(T1, i, i == 0, j, true);
-        }
-      } else {
-        if (n > 1) kv_wait(at_k(1));
-        if (ok && va_elect()) {
-          issue_s(T0, at_k(0) % NS);
-          mma_commit(&kv_empty[at_k(0) % NS]);
-          if (n > 1) {
-            issue_s(T1, at_k(1) % NS);
-            mma_commit(&kv_empty[at_k(1) % NS]);
-          }
-          if (n <= 2) mma_commit(q_empty);
-        }
-        read_named();
-        for (int i = 0; i < n && ok; ++i) {
-          kv_wait(at_v(i));
-          if (i >= ragged && ok) clear(i);
-          const int j = i + 2 < n ? i + 2 : -1;
-          if (j >= 0) kv_wait(at_k(j));
-          if (i & 1) advance(T1, i, i < 2, j, true);
-          else advance(T0, i, i < 2, j, true);
-        }
-      }
-      ring += 2 * n;
-    }
-    if (!ok) *abort_flag = 1;
-    // every MMA issued here has retired before TMEM is released
-    __syncwarp();
-    if (va_elect()) mma_commit(done);
-    mbar_wait_bounded(done, 0, P.err);
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(VA_REGS_SOFTMAX));
     VaWalk<TREE> seg(start, units);
@@ -1040,46 +1040,46 @@ __global__ void __launch_bounds__(256) varlen_join_kernel(const __grid_constant_
     if (f.y) break;
   }
   for (int row = blockIdx.y * ROWS + threadIdx.x / LPR; row < 2 * VA_ROWS; row += ROWS * VA_JOIN_Y) {
-  const int tile = row / VA_ROWS, in_tile = row % VA_ROWS;
-  const int tok = in_tile / P.qpg, i_row = (2 * tail.y + tile) * P.tpt + tok;
-  if (tok >= P.tpt || i_row >= q.n) continue;
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j0 = c; j0 <= last; j0 += BATCH) {
-    float2 ml[BATCH];
-    float4 x[BATCH];
+    const int tile = row / VA_ROWS, in_tile = row % VA_ROWS;
+    const int tok = in_tile / P.qpg, i_row = (2 * tail.y + tile) * P.tpt + tok;
+    if (tok >= P.tpt || i_row >= q.n) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = c; j0 <= last; j0 += BATCH) {
+      float2 ml[BATCH];
+      float4 x[BATCH];
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      const int j = j0 + k;
-      const size_t at = (size_t)(2 * j + (j == c)) * 256 + row;
-      ml[k] = j <= last ? P.part_ml[at] : make_float2(-INFINITY, 0.f);
-      x[k] = j <= last ? *reinterpret_cast<const float4*>(P.part_o + at * HD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < BATCH; ++k) {
+        const int j = j0 + k;
+        const size_t at = (size_t)(2 * j + (j == c)) * 256 + row;
+        ml[k] = j <= last ? P.part_ml[at] : make_float2(-INFINITY, 0.f);
+        x[k] = j <= last ? *reinterpret_cast<const float4*>(P.part_o + at * HD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) mn = fmaxf(mn, ml[k].x);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float f = va_ex2(m - ref);
+      l *= f;
+      o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        if (ml[k].x == -INFINITY) continue;   // no key of this row in the piece (its O may not be written)
+        const float w = va_ex2(ml[k].x - ref);
+        l += ml[k].y * w;
+        o.x += x[k].x * w;
+        o.y += x[k].y * w;
+        o.z += x[k].z * w;
+        o.w += x[k].w * w;
+      }
+      m = mn;
     }
-    float mn = m;
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) mn = fmaxf(mn, ml[k].x);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float f = va_ex2(m - ref);
-    l *= f;
-    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      if (ml[k].x == -INFINITY) continue;   // no key of this row in the piece (its O may not be written)
-      const float w = va_ex2(ml[k].x - ref);
-      l += ml[k].y * w;
-      o.x += x[k].x * w;
-      o.y += x[k].y * w;
-      o.z += x[k].z * w;
-      o.w += x[k].w * w;
-    }
-    m = mn;
-  }
-  const float inv = l > 0.f ? 1.f / l : l;
-  const int h = tail.z * P.qpg + in_tile - tok * P.qpg;
-  const size_t r = (size_t)(q.q0 + i_row);
-  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + r * P.o_row + h * P.o_head + col);
-  *dst = make_uint2(va_pack_out(o.x * inv, o.y * inv, P.out_f16), va_pack_out(o.z * inv, o.w * inv, P.out_f16));
-  if (P.lse && col == 0) P.lse[r * P.n_heads + h] = (m + __log2f(l)) * 0.6931471805599453f;
+    const float inv = l > 0.f ? 1.f / l : l;
+    const int h = tail.z * P.qpg + in_tile - tok * P.qpg;
+    const size_t r = (size_t)(q.q0 + i_row);
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + r * P.o_row + h * P.o_head + col);
+    *dst = make_uint2(va_pack_out(o.x * inv, o.y * inv, P.out_f16), va_pack_out(o.z * inv, o.w * inv, P.out_f16));
+    if (P.lse && col == 0) P.lse[r * P.n_heads + h] = (m + __log2f(l)) * 0.6931471805599453f;
   }
 }
 
