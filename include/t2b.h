@@ -10,7 +10,9 @@
  * workspace (size from the matching *_workspace_bytes query).  It must be
  * zero-filled once before first use (t2b_workspace_init); the kernels leave
  * its counters re-armed for the next call.  Calls that share one workspace
- * must be ordered on one stream.
+ * must be ordered on one stream; the linears may share one whatever their
+ * sizes, every other operation has its own, and the decode attention one for
+ * each set of sizes.
  *
  * Ordering: kernels are launched with programmatic dependent launch.  Each
  * kernel may start reading its (constant) weights before the preceding kernel

@@ -291,13 +291,33 @@ static int pick_kslice(int N, int K, int mblocks) {
   return 256;
 }
 
-static size_t gemv_ws_bytes(int M, int N, int K) {
+// Workspace of the split-K that does not fit a cluster.  The tile counters
+// must be zero before a call and are left zero, so no call may write over
+// another's: they stand in a header of fixed size, at the same place for every
+// shape, and every call's fp32 partials lie behind it.  (Behind the partials
+// their place depended on M: after a call with more rows the counters of one
+// with fewer lay in old partials, and its tiles were never finished.)  A call
+// with more tiles than the header's 16384 (a vocabulary of 151936 from 105 rows
+// on) has its counters behind its partials and clears them itself.
+constexpr size_t GV_HEADER_BYTES = 64 * 1024;
+
+struct GvWorkspace {
+  size_t partial_at, counter_at, counter_bytes, bytes;
+  bool clear;   // the call clears its counters
+};
+static GvWorkspace gemv_workspace(int M, int N, int K) {
+  GvWorkspace w{};
   const int MB = pick_mb(M);
   const int mblocks = (M + MB - 1) / MB;
   const int ksplit = K / pick_kslice(N, K, mblocks);
-  if (ksplit == 1 || gv_cluster(ksplit)) return 0;
-  size_t part = ((size_t)mblocks * ksplit * MB * N * sizeof(float) + 255) & ~size_t(255);
-  return part + (((size_t)mblocks * (N / TILE_N) * sizeof(int) + 255) & ~size_t(255));
+  if (ksplit == 1 || gv_cluster(ksplit)) return w;
+  const size_t part = ((size_t)mblocks * ksplit * MB * N * sizeof(float) + 255) & ~size_t(255);
+  w.counter_bytes = ((size_t)mblocks * (N / TILE_N) * sizeof(int) + 255) & ~size_t(255);
+  w.clear = w.counter_bytes > GV_HEADER_BYTES;
+  w.partial_at = GV_HEADER_BYTES;
+  w.counter_at = w.clear ? GV_HEADER_BYTES + part : 0;
+  w.bytes = GV_HEADER_BYTES + part + (w.clear ? w.counter_bytes : 0);
+  return w;
 }
 
 template <int MB, int CH, int PRO, int EPI, int WFMT>
@@ -325,11 +345,13 @@ static int gemv_launch(LinearParams& p, int pro, int epi, int wfmt, void* ws, si
   const int mblocks = (p.M + MB - 1) / MB;
   p.kslice = pick_kslice(p.N, p.K, mblocks);
   p.ksplit = p.K / p.kslice;
-  const bool need_ws = p.ksplit > 1 && !gv_cluster(p.ksplit);
-  if (ws_bytes < gemv_ws_bytes(p.M, p.N, p.K) || (need_ws && ws == nullptr)) return T2B_ERR_WORKSPACE;
-  size_t part = ((size_t)mblocks * p.ksplit * MB * p.N * sizeof(float) + 255) & ~size_t(255);
-  p.ws_part = reinterpret_cast<float*>(ws);
-  p.ws_cnt = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + part);
+  const GvWorkspace w = gemv_workspace(p.M, p.N, p.K);
+  if (ws_bytes < w.bytes || (w.bytes && ws == nullptr)) return T2B_ERR_WORKSPACE;
+  if (w.bytes) {
+    p.ws_part = reinterpret_cast<float*>(static_cast<char*>(ws) + w.partial_at);
+    p.ws_cnt = reinterpret_cast<int*>(static_cast<char*>(ws) + w.counter_at);
+    if (w.clear && cudaMemsetAsync(p.ws_cnt, 0, w.counter_bytes, st) != cudaSuccess) return T2B_ERR_LAUNCH;
+  }
   const int CH = p.kslice / 256;
   dim3 grid(p.N / TILE_N, p.ksplit, mblocks);
   if (wfmt == T2B_WFMT_QPARAM) {
@@ -410,23 +432,9 @@ static bool use_tc(int M, int N, int K, int wfmt, int x_dtype) {
          tc_supported(M, N, K, wfmt == T2B_WFMT_Q4NX);
 }
 
-// Split of the CUDA-core path's workspace: fp32 partials, then the tile
-// counters (which must be zero before a call).  Zero sizes when the call
-// needs no workspace.
-void linear_workspace_layout(int M, int N, int K, size_t* partial_bytes, size_t* counter_bytes) {
-  *partial_bytes = 0;
-  *counter_bytes = 0;
-  if (M < 1 || N % TILE_N || K % 256 || gemv_ws_bytes(M, N, K) == 0) return;
-  const int MB = pick_mb(M);
-  const int mblocks = (M + MB - 1) / MB;
-  const int ksplit = K / pick_kslice(N, K, mblocks);
-  *partial_bytes = ((size_t)mblocks * ksplit * MB * N * sizeof(float) + 255) & ~size_t(255);
-  *counter_bytes = (((size_t)mblocks * (N / TILE_N) * sizeof(int) + 255) & ~size_t(255));
-}
-
 size_t linear_workspace_bytes(int M, int N, int K) {
   // the path is chosen per call from M; size for the larger so either fits
-  const size_t a = gemv_ws_bytes(M, N, K);
+  const size_t a = gemv_workspace(M, N, K).bytes;
   const size_t b = tc_ws_bytes(M, N, K);
   return a > b ? a : b;
 }
@@ -536,13 +544,16 @@ int gemm_params(const void* weight, const uint32_t* meta, int wfmt, const void* 
 }
 
 // Workspace the path this call takes needs: 0 on the tcgen05 and large-M
-// paths (their split-K stays on chip), the CUDA-core split-K partials and
-// tile counters otherwise (zero when its k-slices meet in a cluster).
-void gemm_path_workspace(const LinearParams& p, int wfmt, size_t* partial_bytes, size_t* counter_bytes) {
-  *partial_bytes = 0;
-  *counter_bytes = 0;
-  if (use_prefill(p.M, wfmt, p.x_dtype) || use_tc(p.M, p.N, p.K, wfmt, p.x_dtype)) return;
-  linear_workspace_layout(p.M, p.N, p.K, partial_bytes, counter_bytes);
+// paths (their split-K stays on chip), the CUDA-core split-K's otherwise (zero
+// when its k-slices meet in a cluster).  `counter_bytes` at `counter_at` must
+// be zero before the call.
+size_t gemm_path_workspace(const LinearParams& p, int wfmt, size_t* counter_at, size_t* counter_bytes) {
+  *counter_at = *counter_bytes = 0;
+  if (use_prefill(p.M, wfmt, p.x_dtype) || use_tc(p.M, p.N, p.K, wfmt, p.x_dtype)) return 0;
+  const GvWorkspace w = gemv_workspace(p.M, p.N, p.K);
+  *counter_at = w.counter_at;
+  *counter_bytes = w.counter_bytes;
+  return w.bytes;
 }
 
 int gemm_launch(LinearParams& p, int wfmt, void* ws, size_t ws_bytes, cudaStream_t st) {

@@ -29,7 +29,7 @@
 
 namespace t2b {
 
-constexpr size_t NOALLOC_SCRATCH_BYTES = size_t(8) << 20;
+constexpr size_t NOALLOC_SCRATCH_BYTES = (size_t(8) << 20) + 64 * 1024;   // 8 MiB of partials, and the counters
 
 // The array's name is a host-side stand-in in host code; its device address
 // comes from cudaGetSymbolAddress below.
@@ -66,16 +66,15 @@ extern "C" T2B_API int t2b_w4a16_gemm_noalloc(const void* weight, const uint32_t
   const int r = t2b::gemm_params(weight, meta, wfmt, x, x_dtype, y, y_dtype, M, N, K, group_size, &p);
   if (r != T2B_OK) return r;
   // scratch only for the path this call takes (the tcgen05 and large-M paths need none)
-  size_t partial_bytes = 0, counter_bytes = 0;
-  t2b::gemm_path_workspace(p, wfmt, &partial_bytes, &counter_bytes);
-  if (partial_bytes + counter_bytes > t2b::NOALLOC_SCRATCH_BYTES) return T2B_ERR_WORKSPACE;
+  size_t counter_at = 0, counter_bytes = 0;
+  if (t2b::gemm_path_workspace(p, wfmt, &counter_at, &counter_bytes) > t2b::NOALLOC_SCRATCH_BYTES) return T2B_ERR_WORKSPACE;
   void* scratch = nullptr;
   const int st = t2b::scratch_on_current_device(&scratch);
   if (st != T2B_OK) return st;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (counter_bytes) {
     // split-K tile counters must start at zero (an earlier aborted call may have left them armed)
-    if (cudaMemsetAsync(static_cast<char*>(scratch) + partial_bytes, 0, counter_bytes, s) != cudaSuccess)
+    if (cudaMemsetAsync(static_cast<char*>(scratch) + counter_at, 0, counter_bytes, s) != cudaSuccess)
       return T2B_ERR_LAUNCH;
   }
   return t2b::gemm_launch(p, wfmt, scratch, t2b::NOALLOC_SCRATCH_BYTES, s);
