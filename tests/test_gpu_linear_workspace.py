@@ -82,3 +82,13 @@ def test_draft_trees_behind_a_packed_prompt(nodes):
         states.append((log, [t.clone() for t in eng.k_cache + eng.v_cache]))
     assert states[0][0] == states[1][0]
     assert all(torch.equal(a, b) for a, b in zip(states[0][1], states[1][1]))
+
+
+def test_a_tree_of_fewer_rows_than_the_prompt_needs_more_partials():
+    """64 rows run in k-slices twice as large as 48 do: the smaller call's workspace is the larger."""
+    model, g = synth.random_model(CFG, seed=31), torch.Generator().manual_seed(32)
+    eng = DecodeEngine(CFG, model, batch=2, max_ctx=128, use_graph=False)
+    eng.prefill_packed([torch.randint(0, CFG.vocab_size, (n,), generator=g) for n in (40, 24)])
+    tok = np.repeat(eng.tokens.cpu().numpy()[:, None], 24, 1)
+    _, count, _ = eng.decode_tree(tok, np.tile(np.arange(-1, 23), (2, 1)))
+    assert (count >= 1).all()

@@ -30,6 +30,8 @@
 
 #include <stdlib.h>
 
+#include <algorithm>
+
 namespace t2b {
 
 constexpr int GV_THREADS = 256;
@@ -283,11 +285,12 @@ static int pick_mb(int M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
 // k-slice per CTA: the smallest of 256/512/1024 that keeps a tile's k-slices
 // within one cluster (<= 8), else 256/512 with the grid at about 1-4 CTAs
 // per SM (workspace split-K).
+constexpr long SMALL_SLICE_CTAS = 4L * 148;
 static int pick_kslice(int N, int K, int mblocks) {
   for (int ks : {256, 512, 1024})
     if (K % ks == 0 && K / ks <= GV_MAX_CLUSTER) return ks;
   const long tiles = (long)(N / TILE_N) * mblocks;
-  if (K % 512 == 0 && tiles * (K / 256) > 4L * 148) return 512;
+  if (K % 512 == 0 && tiles * (K / 256) > SMALL_SLICE_CTAS) return 512;
   return 256;
 }
 
@@ -432,11 +435,15 @@ static bool use_tc(int M, int N, int K, int wfmt, int x_dtype) {
          tc_supported(M, N, K, wfmt == T2B_WFMT_Q4NX);
 }
 
+// What a call of M rows or fewer needs, on either path (buffers kept for a long
+// pass serve shorter ones).  The partials grow with the row blocks except where
+// pick_kslice goes over to slices of twice the size: there a call of fewer rows
+// needs up to twice as much, the most at the last row block of the small slices.
 size_t linear_workspace_bytes(int M, int N, int K) {
-  // the path is chosen per call from M; size for the larger so either fits
-  const size_t a = gemv_workspace(M, N, K).bytes;
-  const size_t b = tc_ws_bytes(M, N, K);
-  return a > b ? a : b;
+  const size_t a = std::max(gemv_workspace(M, N, K).bytes, tc_ws_bytes(M, N, K));
+  const long per_block = (long)(N / TILE_N) * (K / 256);
+  const long blocks = per_block > 0 ? SMALL_SLICE_CTAS / per_block : 0;
+  return blocks >= 1 && 8 * blocks < M ? std::max(a, gemv_workspace((int)(8 * blocks), N, K).bytes) : a;
 }
 
 int linear_launch(LinearParams& p, int pro, int epi, int wfmt, void* ws, size_t ws_bytes, cudaStream_t st) {
