@@ -1,0 +1,117 @@
+"""The serving operators at sizes, values and calls that their first tests do not reach."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_serving import gen, ints, randn
+from torch2iron_b200.operators import DraftTreeAttention, PackedAttention, draft_tree
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+# ---------------------------------------------------------------------------
+# scores so large that neighbouring fp32 values are units apart
+# ---------------------------------------------------------------------------
+def run_packed(q, k, v, scale):
+    n, nh, hd = q.shape
+    nkv = k.shape[1]
+    out, lse = torch.empty_like(q), torch.empty(n, nh, device="cuda")
+    PackedAttention(tokens=n, num_seqs=1, num_kv_groups=nkv, q_heads_per_group=nh // nkv, head_dim=hd, dtype=q.dtype,
+                    scale=scale)(q, k, v, ints([0, n]), out, lse=lse)
+    return out, lse
+
+
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 24, 3e7, 6e7, 1.1e8, 2.0 ** 28, 7e8, 3e9])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_equal_scores_of_any_size_give_the_mean(size, dtype):
+    """Equal keys: every weight is the same, whatever the scores' rounding, so row
+    i is the mean of v[0..i]: a weight is at most half a step of its type off (u),
+    the sum and the result's rounding as in ``assert_attention``."""
+    n, hd = 300, 64
+    a = math.sqrt(size * math.log(2.0))                       # scores of about size in powers of two
+    q = torch.zeros(n, 2, hd, device="cuda", dtype=dtype)
+    q[:, :, :3] = torch.tensor([a, a / 700, -a / 900])
+    q[::2] *= -1
+    k = torch.zeros(n, 1, hd, device="cuda", dtype=dtype)
+    k[:, :, :3] = torch.tensor([a, a / 3, a / 7])
+    v = randn(gen(1), n, 1, hd, dtype=dtype)
+    out, lse = run_packed(q, k, v, 1.0)
+    u = torch.finfo(dtype).eps / 2
+    i = torch.arange(1, n + 1, dtype=torch.float64)[:, None, None]
+    mean = v.double().cpu().cumsum(0) / i
+    off = v.double().cpu().abs().cumsum(0) / i * (u + (300 + 4) * 2.0 ** -24)
+    got = out.double().cpu()
+    assert torch.isfinite(got).all() and torch.isfinite(lse).all()
+    assert ((got - mean).abs() <= off + u * (mean.abs() + off).clamp(min=torch.finfo(dtype).tiny) + 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("base,step", [(2.0 ** 24, 2.0), (2.0 ** 25, 4.0), (2.0 ** 26, 8.0), (2.0 ** 27, 16.0),
+                                       (-(2.0 ** 27), 16.0), (2.0 ** 28, 32.0)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scores_that_rise_by_their_own_spacing(base, step, dtype):
+    """Scores base + step * (block of 128 keys), exact in fp32, in powers of two:
+    the reference of the exponents has to follow a rise that its own rounding
+    nearly hides.  The weights are powers of two, so only sums and the result round."""
+    n, hd = 700, 64
+    scale = float(np.float32(math.log(2.0)))
+    assert np.float32(scale) * np.float32(1.4426950408889634) == 1.0
+    q = torch.zeros(n, 1, hd)
+    k = torch.zeros(n, 1, hd)
+    q[:, 0, 0], k[:, 0, 0] = 2.0 ** 14, base / 2.0 ** 14
+    q[:, 0, 1] = step
+    block = torch.arange(n) // 128
+    k[:, 0, 1] = block.float()
+    q, k, v = q.to(dtype).cuda(), k.to(dtype).cuda(), randn(gen(2), n, 1, hd, dtype=dtype)
+    out, _ = run_packed(q, k, v, scale)
+    w = torch.exp2(step * (block[None] - block[:, None]).double()).tril()
+    want = (w @ v[:, 0].double().cpu()) / w.sum(1, keepdim=True)
+    size = (w @ v[:, 0].double().cpu().abs()) / w.sum(1, keepdim=True)
+    u = torch.finfo(dtype).eps / 2
+    off = size * (700 + 8) * 2.0 ** -24 + (2.0 ** -32 * 700 if dtype == HF else 0.0) * 8
+    got = out[:, 0].double().cpu()
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= off + u * (want.abs() + off).clamp(min=torch.finfo(dtype).tiny) + 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("dtype,q_scale", [(HF, 3000.0), (BF, 1e4), (BF, 1e6)])
+def test_huge_random_scores_stay_inside_the_values(dtype, q_scale):
+    """Scores whose own rounding exceeds a power of two: which key wins is open, the result is finite and between
+    the least and the largest value seen."""
+    n, hd = 500, 128
+    q, k = randn(gen(3), n, 4, hd, dtype=dtype, scale=q_scale), randn(gen(4), n, 2, hd, dtype=dtype, scale=q_scale)
+    v = randn(gen(5), n, 2, hd, dtype=dtype)
+    out, lse = run_packed(q, k, v, 1.0)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    low, high = (f(v.float(), 0).values.repeat_interleave(2, 1) for f in (torch.cummin, torch.cummax))
+    slack = 2 * torch.finfo(dtype).eps * v.float().abs().max()
+    assert (out.float() >= low - slack).all() and (out.float() <= high + slack).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** 20, 1.1e8, 3e9])
+@pytest.mark.parametrize("ctx", [100, 5000])
+def test_equal_scores_of_any_size_over_a_cache(size, ctx):
+    """The same for a tree whose items have one tile and are cut between CTAs: bounds as above."""
+    T, hd, a = 20, 64, math.sqrt(size * math.log(2.0))
+    one = torch.tensor([a, a / 3, a / 7])
+    q, k, v = torch.zeros(1, T, 2, hd), torch.zeros(1, 1, 5056, hd), randn(gen(6), 1, 1, 5056, hd, dtype=HF)
+    q[..., :3], k[..., :3] = one, one
+    q[:, ::3] *= -1
+    q, k = q.half().cuda(), k.half().cuda()
+    kd, vd = k[:, :, :T].transpose(1, 2).contiguous(), randn(gen(7), 1, T, 1, hd, dtype=HF)
+    mask, _ = draft_tree(np.arange(-1, T - 1)[None])
+    out, lse = torch.empty_like(q), torch.empty(1, T, 2, device="cuda")
+    DraftTreeAttention(batch=1, nodes=T, max_ctx=5056, num_kv_groups=1, q_heads_per_group=2, dtype=HF, scale=1.0)(
+        q, k, v, kd, vd, ints([ctx]), mask.cuda(), out, lse=lse)
+    seen = torch.cat([v[0, 0, :ctx], vd[0, :, 0]]).double().cpu()
+    n = torch.arange(ctx + 1, ctx + T + 1, dtype=torch.float64)[:, None]
+    mean, size_of = seen.cumsum(0)[ctx:] / n, seen.abs().cumsum(0)[ctx:] / n
+    u = 2.0 ** -11
+    off = size_of * (u + (ctx + 40) * 2.0 ** -24)
+    got = out[0].double().cpu()
+    assert torch.isfinite(lse).all()
+    assert ((got - mean[:, None]).abs() <= (off + u * (mean.abs() + off).clamp(min=2.0 ** -14) + 2.0 ** -30)[:, None]).all()

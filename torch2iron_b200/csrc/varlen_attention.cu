@@ -49,9 +49,15 @@
 // once, to the operands' 16-bit type, as A of the second product (the sum
 // uses them before rounding).  The exponent's reference m is moved, and O
 // rescaled, only when a row's maximum outgrows it: it starts VA_HEAD below the
-// first block's maximum and moves when a score passes m + VA_ROOM, so a weight
-// is at most 2^15 (in fp16 range) and the largest is at least 2^VA_HEAD of the
-// time it was set, which keeps small fp16 weights 2^7 further from underflow.
+// first block's maximum and moves when a score is more than VA_ROOM above it,
+// and the largest weight is at least 2^VA_HEAD of the time it was set, which
+// keeps small fp16 weights 2^7 further from underflow.  An exponent is one FMA
+// of the score, so it can exceed the rounded difference that was compared by
+// half the spacing of fp32 values there: below 2^23 a weight is at most 2^15.5,
+// in fp16 range.  A row whose m lies further out takes the branch that moves m
+// at every block, and there its scores are scaled and rounded as the maximum
+// was, and written back less m (over the scale, which the FMA multiplies by): a
+// weight is at most 2^15 and the largest of a block that moved m at least 1.
 //
 // Every mbarrier wait is time-bounded (T2B_ERR_TIMEOUT in the status word,
 // then every role stops at its next wait).
@@ -80,6 +86,7 @@ constexpr int VA_ITEM = 4;              // units an item costs beside its blocks
 constexpr int VA_SNAP = 8;              // items of up to this many blocks stay in one CTA
 constexpr int VA_MIN_UNITS = 5;         // units per CTA, at least
 constexpr float VA_HEAD = 7.f, VA_ROOM = 15.f;
+constexpr float VA_FAR = 8388608.f;     // 2^23: from here on fp32 values are 1 and more apart
 
 struct VaParams {
   CUtensorMap qmap;                     // (hd, heads, rows), box (64, qpg, tokens per tile)
@@ -797,6 +804,7 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
       const int tile_limit = TREE ? seg.q.avail : va_limit(seg.q, (2 * seg.p + tile) * tpt);
       const int step = seg.dual ? 1 : 2, n = seg.dual ? (t ? seg.n : seg.n0) : seg.n;
       float m = -INFINITY, l = 0.f;
+      float limit_m = -INFINITY, ref = 0.f;   // a greater score moves m; what the exponents subtract
       bool any = false;
       for (int i = seg.dual ? 0 : t; i < n && ok; i += step) {
         const int b = seg.b0 + i, kb = b * VA_ROWS;
@@ -836,7 +844,7 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
         if (!ok) s_bad[pair] = 1;
         // (behind this barrier both halves hold their scores; a row that is not live
         // holds whatever was there, and must not decide when its neighbours rescale)
-        if (va_pair_any(bar, (live && top > m + VA_ROOM) || !ok)) {
+        if (va_pair_any(bar, (live && top > limit_m) || !ok)) {
           if (u) *x_slot = top;
           va_pair_sync(bar);
           if (s_bad[pair]) {
@@ -861,11 +869,27 @@ __global__ void __launch_bounds__(VA_THREADS, 1) varlen_attention_kernel(const _
             tmem_st_wait();
           }
           m = mn;
+          const bool far = live && fabsf(m) >= VA_FAR && m != -INFINITY;
+          limit_m = far ? -INFINITY : __fadd_rd(m, VA_ROOM);   // (rounded down: the comparison is exact)
+          ref = far || m == -INFINITY ? 0.f : m;
+          if (__any_sync(0xffffffffu, far)) {   // a far row's scores become differences from m (see Numerics)
+            const float per = 1.f / scale;
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) {
+              uint32_t s[16];
+              tmem_ld16(s_col + k * 16, s);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (far) s[e] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(s[e]), scale), m) * per);
+              tmem_st16(s_col + k * 16, s);
+            }
+            tmem_st_wait();
+          }
           tc_fence_before();
           va_pair_sync(bar);   // both halves of O are ready before either half of P is announced
         }
         any = true;
-        const float ref = m == -INFINITY ? 0.f : m;
         const f32x2 scale2 = va_pair(scale, scale), ref2 = va_pair(-ref, -ref);
         f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
