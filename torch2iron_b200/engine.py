@@ -619,7 +619,9 @@ class DecodeEngine:
         With ``score`` every position's distribution is evaluated as well and a
         :class:`PromptScores` is returned: the log probability of each prompt
         token after the first, the entropy at every position and the
-        ``num_top`` most likely next tokens there."""
+        ``num_top`` most likely next tokens there.  A timed-out device wait then
+        raises here; without ``score`` ``check_device_errors`` reports it, as
+        after ``prefill``."""
         from .operators import TokenLogProbs
         ids = self._packed_prompts(prompts)
         if not 0 <= num_top <= min(32, self.cfg.vocab_size):
@@ -688,6 +690,8 @@ class DecodeEngine:
                         top_logprob=out["top_logprob"][o:o + n] if num_top else None,
                         top_index=out["top_index"][o:o + n] if num_top else None)
             self._enqueue_head(st)
+        if score:
+            self.check_device_errors()                        # scores behind a timed-out wait are not returned
         self.tokens.copy_(self.next_tokens)
         self.pos.copy_(torch.from_numpy(lens.astype(np.int32)))
         return None if out is None else PromptScores(lens.tolist(), **out)
@@ -719,6 +723,8 @@ class DecodeEngine:
         the model's own greedy token: its K/V rows move into the cache
         (``t2b_tree_commit``) and the row continues behind it.  A row without live
         nodes, or without room in the cache, is left as it is.
+
+        A timed-out device wait raises and leaves every row where it was.
 
         Returns host int32 tensors ``(path [B, T], num_accepted [B], next_tokens
         [B])``: the accepted nodes (-1 behind them; the row emitted the tokens of
@@ -773,11 +779,13 @@ class DecodeEngine:
             _lib.check("t2b_tree_commit", L.t2b_tree_commit(
                 p(tb["tree"][0]), p(tb["tree"][1]), p(tb["predicted"]), p(self.pos), p(tb["live"]), *layers, cfg.n_layers,
                 p(tb["path"]), p(count), p(following), p(length), B, T, nkv, hd, ctx, *drafted, *drafted, st))
+        path, walk = tb["path"].cpu(), tb["walk"].cpu()
+        # Before the rows move: a step with a timed-out wait can be repeated (what
+        # it wrote into the caches lies behind the rows' positions).
+        self.check_device_errors()
         self.pos.copy_(length)
         self.tokens.copy_(torch.where(count > 0, following, self.tokens))
         self.next_tokens.copy_(self.tokens)
-        path, walk = tb["path"].cpu(), tb["walk"].cpu()
-        self.check_device_errors()
         return path, walk[0].clone(), walk[1].clone()
 
     def generate(self, prompts: torch.Tensor, new_tokens: int, stepwise_prefill: bool = False,
