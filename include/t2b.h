@@ -450,6 +450,11 @@ T2B_API size_t t2b_varlen_attention_workspace_bytes(int head_dim);
  *   kv_seqs >= n_seqs: cache form [kv_seqs][n_kv][kv_tokens][head_dim]
  *     (strides k_seq, k_head, k_tok, ..); key j of sequence s is row j of
  *     cache row s.  k_start is NULL, k_len is given.
+ * The work is counted in 32 bits: a call that could exceed 2^31 - 1 units is
+ * refused (T2B_ERR_SHAPE).  A unit is 128 keys for 128 / (n_heads / n_kv)
+ * query rows of one kv head; the host's bound takes kv_tokens keys for every
+ * row where k_len is given, else one prompt of all total_q rows (32 over 8
+ * heads: prompts up to 1.4 million tokens).
  */
 T2B_API int t2b_packed_attention(const void* q, const void* k, const void* v, void* out, float* lse, int dtype,
                                  int out_dtype, const int32_t* q_start, const int32_t* k_start, const int32_t* k_len,

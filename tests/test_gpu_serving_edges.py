@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from tests.serving_ref import assert_attention, attention_rows
 from tests.test_gpu_serving import gen, ints, randn
 from torch2iron_b200.operators import DraftTreeAttention, PackedAttention, draft_tree
 
@@ -115,3 +116,21 @@ def test_equal_scores_of_any_size_over_a_cache(size, ctx):
     got = out[0].double().cpu()
     assert torch.isfinite(lse).all()
     assert ((got - mean[:, None]).abs() <= (off + u * (mean.abs() + off).clamp(min=2.0 ** -14) + 2.0 ** -30)[:, None]).all()
+
+
+# ---------------------------------------------------------------------------
+# many sequences
+# ---------------------------------------------------------------------------
+def test_packed_half_a_million_tokens_of_short_prompts():
+    """32768 prompts of 16 tokens over 8 key heads: some of them against the reference, each row finite."""
+    S, n, nh, hd = 32768, 16, 8, 64
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, k, v = (torch.randn(S * n, nh, hd, generator=g, device="cuda").to(BF) for _ in range(3))
+    out, lse = torch.full_like(q, math.nan), torch.full((S * n, nh), math.nan, device="cuda")
+    op = PackedAttention(tokens=S * n, num_seqs=S, num_kv_groups=nh, q_heads_per_group=1, head_dim=hd)
+    op(q, k, v, torch.arange(0, S * n + 1, n, dtype=torch.int32, device="cuda"), out, lse=lse)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    seen = torch.arange(n)[None] <= torch.arange(n)[:, None]
+    for s in (0, 1, 639, 640, 641, 10007, S - 1):
+        r = slice(s * n, (s + 1) * n)
+        assert_attention(out[r], lse[r], attention_rows(q[r], k[r], v[r], seen, op.scale))

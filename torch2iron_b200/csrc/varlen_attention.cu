@@ -1113,6 +1113,7 @@ __global__ void __launch_bounds__(256) varlen_join_kernel(const __grid_constant_
 static bool va_misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 constexpr int VA_MAX_CTAS = 148;
+constexpr int VA_MAX_KEYS = 0x7fff0000;   // (positions plus a block stay in an int)
 
 static int va_host_blocks(int keys) { return (keys + VA_ROWS - 1) / VA_ROWS; }
 
@@ -1153,11 +1154,29 @@ static int va_launch_t(VaParams& P, int grid, bool join, cudaStream_t st) {
   return launch_pdl(varlen_join_kernel<HD, TREE>, dim3(grid, VA_JOIN_Y), dim3(256), 0, st, P, grid);
 }
 
-// max_blocks: no item has more blocks of keys; pairs: no more (sequence, pair of tiles).
-static int va_launch(VaParams& P, int hd, bool f16, const void* q, size_t q_row, size_t q_head, long long pairs,
-                     long long max_blocks, void* ws, size_t ws_bytes, cudaStream_t st) {
+// Upper bounds of a call's units, which the kernel counts in 32 bits.  The host
+// knows no length: `pairs` bounds the pairs of tiles of all sequences, and each
+// may see all keys there are.
+static double va_most_units(double pairs, int max_blocks, int n_kv) {
+  return pairs * (2.0 * max_blocks + VA_ITEM) * n_kv;
+}
+// Prompts over their own packed keys: pair p of a prompt sees 2 tpt (p + 1) keys
+// at most, so a prompt of x pairs has tpt / 64 x (x + 1) units of keys and
+// (2 + VA_ITEM) x more, and all prompts together no more than one of all rows
+// has beside the short ones' first pairs.
+static double va_most_units_own(int rows, double seqs, int tpt, int n_kv) {
+  const double x = rows / (2 * tpt) + 1;
+  return (tpt / 64.0 * (x * x + 3 * x + 2 * seqs) + (2 + VA_ITEM) * (x + seqs)) * n_kv;
+}
+
+// units: no more of them; max_blocks: no item has more blocks of keys.
+static int va_check_sizes(int hd, double units, const void* ws, size_t ws_bytes) {
+  if (units > 2147483647.0) return T2B_ERR_SHAPE;
   if (!ws || ws_bytes < va_ws_bytes(hd)) return T2B_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(ws) & 255) return T2B_ERR_ALIGN;
+  return reinterpret_cast<uintptr_t>(ws) & 255 ? T2B_ERR_ALIGN : T2B_OK;
+}
+static int va_launch(VaParams& P, int hd, bool f16, const void* q, size_t q_row, size_t q_head, double units,
+                     int max_blocks, void* ws, cudaStream_t st) {
   P.head = static_cast<int4*>(ws);
   P.part_ml = reinterpret_cast<float2*>(P.head + 2 * VA_MAX_CTAS);
   P.part_o = reinterpret_cast<float*>(P.part_ml + 2 * VA_MAX_CTAS * 256);
@@ -1168,9 +1187,7 @@ static int va_launch(VaParams& P, int hd, bool f16, const void* q, size_t q_row,
   int dev = 0, sms = VA_MAX_CTAS;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return T2B_ERR_LAUNCH;
-  const long long units = pairs * (2 * max_blocks + VA_ITEM) * P.n_kv;
-  if (units > 0x7fffffffll) return T2B_ERR_SHAPE;
-  const int grid = (int)std::max(1ll, std::min<long long>({units / VA_MIN_UNITS, sms, VA_MAX_CTAS}));
+  const int grid = std::max(1, std::min({(int)(units / VA_MIN_UNITS), sms, VA_MAX_CTAS}));
   const bool join = grid > 1 && max_blocks > VA_SNAP;
   const bool tree = P.T > 0;
   if (hd == 128) {
@@ -1196,7 +1213,7 @@ static int va_check(const void* q, const void* k, const void* v, const void* out
     return T2B_ERR_ARG;
   if (!(scale > 0.f) || !isfinite(scale)) return T2B_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return T2B_ERR_SHAPE;
-  if (rows < 1 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || n_heads / n_kv > 128) return T2B_ERR_SHAPE;
+  if (rows < 1 || rows > VA_MAX_KEYS || n_kv < 1 || n_heads < 1 || n_heads % n_kv || n_heads / n_kv > 128) return T2B_ERR_SHAPE;
   if (va_misaligned(q) || va_misaligned(k) || va_misaligned(v) || va_misaligned(out)) return T2B_ERR_ALIGN;
   for (size_t s : strides)
     if (s % 8 || s == 0) return T2B_ERR_ALIGN;
@@ -1214,7 +1231,7 @@ extern "C" int t2b_packed_attention(const void* q, const void* k, const void* v,
                           {q_row, q_head, o_row, o_head, k_tok, k_head, k_seq, v_tok, v_head, v_seq});
   if (rc != T2B_OK) return rc;
   if (!q_start) return T2B_ERR_ARG;
-  if (n_seqs < 1 || kv_tokens < 1 || kv_seqs < 0) return T2B_ERR_SHAPE;
+  if (n_seqs < 1 || n_seqs > VA_MAX_KEYS || kv_tokens < 1 || kv_tokens > VA_MAX_KEYS || kv_seqs < 0) return T2B_ERR_SHAPE;
   if (kv_seqs ? (kv_seqs < n_seqs || !k_len || k_start) : (k_start == nullptr) != (k_len == nullptr)) return T2B_ERR_ARG;
   VaParams P{};
   const bool f16 = dtype == T2B_DTYPE_F16;
@@ -1223,14 +1240,19 @@ extern "C" int t2b_packed_attention(const void* q, const void* k, const void* v,
   P.tpt = VA_ROWS / P.qpg;
   P.o_row = o_row, P.o_head = o_head;
   P.kv_tokens = kv_tokens, P.cached = kv_seqs > 0;
+  const int max_blocks = va_host_blocks(kv_tokens);
+  const double live = std::min(n_seqs, total_q);   // sequences with rows
+  double units = va_most_units(total_q / (2 * P.tpt) + live, max_blocks, n_kv);
+  if (!k_len) units = std::min(units, va_most_units_own(total_q, live, P.tpt, n_kv));
+  const int sized = va_check_sizes(head_dim, units, workspace, workspace_bytes);
+  if (sized != T2B_OK) return sized;
   const size_t seqs = kv_seqs ? kv_seqs : 1;
   if (!va_kv_map(&P.kmap, f16, k, head_dim, kv_tokens, n_kv, seqs, k_tok, k_head, k_seq) ||
       !va_kv_map(&P.vmap, f16, v, head_dim, kv_tokens, n_kv, seqs, v_tok, v_head, v_seq))
     return T2B_ERR_ARG;
   P.q_start = q_start, P.k_start = k_start, P.k_len = k_len;
   P.scale_log2 = scale * 1.4426950408889634f;
-  return va_launch(P, head_dim, f16, q, q_row, q_head, total_q / (2 * P.tpt) + (long long)n_seqs,
-                   std::max(1, va_host_blocks(kv_tokens)), workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+  return va_launch(P, head_dim, f16, q, q_row, q_head, units, max_blocks, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int t2b_tree_attention(const void* q, const void* k_cache, const void* v_cache, const void* k_draft,
@@ -1240,7 +1262,8 @@ extern "C" int t2b_tree_attention(const void* q, const void* k_cache, const void
                                   size_t o_row, size_t o_head, size_t kd_row, size_t kd_node, size_t kd_head,
                                   size_t vd_row, size_t vd_node, size_t vd_head, float scale, void* workspace,
                                   size_t workspace_bytes, void* stream) {
-  if (B < 1 || T < 1 || T > VA_MAX_NODES || max_ctx < 1 || (long long)B * T > 0x7fffffffll) return T2B_ERR_SHAPE;
+  if (B < 1 || T < 1 || T > VA_MAX_NODES || max_ctx < 1 || max_ctx > VA_MAX_KEYS || (long long)B * T > VA_MAX_KEYS)
+    return T2B_ERR_SHAPE;
   const int rc = va_check(q, k_cache, v_cache, out, dtype, out_dtype, B * T, n_heads, n_kv, head_dim, scale,
                           {q_row, q_head, o_row, o_head, kd_row, kd_node, kd_head, vd_row, vd_node, vd_head});
   if (rc != T2B_OK) return rc;
@@ -1257,13 +1280,15 @@ extern "C" int t2b_tree_attention(const void* q, const void* k_cache, const void
   P.mask = reinterpret_cast<const uint32_t*>(mask);
   P.T = T, P.words = (T + 63) / 64;
   P.scale_log2 = scale * 1.4426950408889634f;
+  const int max_blocks = va_host_blocks(max_ctx) + va_host_blocks(T);
+  const double units = va_most_units((double)B * ((T + 2 * P.tpt - 1) / (2 * P.tpt)), max_blocks, n_kv);
+  const int sized = va_check_sizes(head_dim, units, workspace, workspace_bytes);
+  if (sized != T2B_OK) return sized;
   const size_t head = (size_t)max_ctx * head_dim;
   if (!va_kv_map(&P.kmap, f16, k_cache, head_dim, max_ctx, n_kv, B, head_dim, head, n_kv * head) ||
       !va_kv_map(&P.vmap, f16, v_cache, head_dim, max_ctx, n_kv, B, head_dim, head, n_kv * head) ||
       !va_kv_map(&P.kdmap, f16, k_draft, head_dim, T, n_kv, B, kd_node, kd_head, kd_row) ||
       !va_kv_map(&P.vdmap, f16, v_draft, head_dim, T, n_kv, B, vd_node, vd_head, vd_row))
     return T2B_ERR_ARG;
-  return va_launch(P, head_dim, f16, q, q_row, q_head, (long long)B * ((T + 2 * P.tpt - 1) / (2 * P.tpt)),
-                   va_host_blocks(max_ctx) + va_host_blocks(T), workspace, workspace_bytes,
-                   reinterpret_cast<cudaStream_t>(stream));
+  return va_launch(P, head_dim, f16, q, q_row, q_head, units, max_blocks, workspace, reinterpret_cast<cudaStream_t>(stream));
 }

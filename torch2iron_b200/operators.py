@@ -491,7 +491,9 @@ class PackedAttention:
     are cache rows ``[num_seqs, num_kv_groups, max_ctx, head_dim]`` and ``k_len``
     says how many of each row count, the sequence's own queries among them.
     A query without keys gets zeros (and ``lse`` -inf); rows of ``out`` and
-    ``lse`` outside every sequence keep what they held."""
+    ``lse`` outside every sequence keep what they held.  A call that could have
+    more than 2^31 - 1 units of work (``t2b_packed_attention``; one prompt of 1.4
+    million tokens at 32 over 8 heads) is refused."""
 
     tokens: int
     num_seqs: int
