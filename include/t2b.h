@@ -429,6 +429,9 @@ T2B_API int t2b_argmax_rows(const void* logits, int dtype, int M, int V, int ld,
  * other rows of its sequence too (0 times it is not 0).  The lengths, starts and masks are read on
  * the device; what lies outside the given extents is ignored (clamped), and
  * output rows that belong to no sequence or to no live node are not written.
+ * out and lse share no memory with q, K, V or one another (T2B_ERR_ARG), except
+ * that out may be q itself, with q's strides; views that interleave (heads of
+ * one wider tensor) are told apart where they have their strides in common.
  * The workspace (t2b_varlen_attention_workspace_bytes) needs no
  * initialisation and is 256-byte aligned; calls that share one must be
  * ordered on one stream.
@@ -493,9 +496,9 @@ T2B_API int t2b_tree_attention(const void* q, const void* k_cache, const void* v
  * n_accepted[b].  A row with n_nodes[b] <= 0 or ctx_len[b] outside
  * [0, max_ctx) accepts nothing (next_token -1, new_len = ctx_len).  Every
  * other cache row stays as it is.  k_draft .. v_cache are HOST arrays of
- * n_layers device pointers; drafts and caches must not overlap.  The results
- * (path .. new_len) must not overlap the inputs nor one another (new_len is not
- * ctx_len: T2B_ERR_ARG).
+ * n_layers device pointers.  The caches and the results (path .. new_len) share
+ * no memory with the inputs nor with one another, a draft's memory reaching from
+ * its first element to its last (T2B_ERR_ARG).
  */
 T2B_API int t2b_tree_commit(const int32_t* tokens, const int32_t* parents, const int32_t* predicted,
                             const int32_t* ctx_len, const int32_t* n_nodes, const void* const* k_draft,

@@ -8,7 +8,7 @@ import torch
 
 from tests.serving_ref import assert_attention, attention_rows
 from tests.test_gpu_serving import gen, ints, randn
-from torch2iron_b200.operators import DraftTreeAttention, PackedAttention, draft_tree
+from torch2iron_b200.operators import DraftTreeAttention, DraftTreeCommit, PackedAttention, draft_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,45 @@ def test_packed_half_a_million_tokens_of_short_prompts():
     for s in (0, 1, 639, 640, 641, 10007, S - 1):
         r = slice(s * n, (s + 1) * n)
         assert_attention(out[r], lse[r], attention_rows(q[r], k[r], v[r], seen, op.scale))
+
+
+# ---------------------------------------------------------------------------
+# results over inputs
+# ---------------------------------------------------------------------------
+def test_attention_in_place_of_q_gives_the_same_bits():
+    g, n, nh, nkv, hd = gen(60), [700, 1, 90, 1500], 8, 2, 64
+    total, start = sum(n), np.concatenate([[0], np.cumsum(n)])
+    fused = randn(g, total, nh + 2 * nkv, hd)
+    q, k, v = fused[:, :nh], fused[:, nh:nh + nkv], fused[:, nh + nkv:]
+    op = PackedAttention(tokens=total, num_seqs=4, num_kv_groups=nkv, q_heads_per_group=4, head_dim=hd)
+    out, keys = torch.empty(total, nh, hd, dtype=BF, device="cuda"), fused[:, nh:].clone()
+    op(q, k, v, ints(start), out)
+    op(q, k, v, ints(start), q)
+    assert torch.equal(q, out) and torch.equal(fused[:, nh:], keys)
+    B, T = 2, 40
+    q, kd, vd = randn(g, B, T, nh, hd), randn(g, B, T, nkv, hd), randn(g, B, T, nkv, hd)
+    kc, vc = randn(g, B, nkv, 4096, hd), randn(g, B, nkv, 4096, hd)
+    mask, _ = draft_tree(np.tile(np.arange(-1, T - 1), (B, 1)))
+    op = DraftTreeAttention(batch=B, nodes=T, max_ctx=4096, num_kv_groups=nkv, q_heads_per_group=4, head_dim=hd)
+    out = torch.empty_like(q)
+    op(q, kc, vc, kd, vd, ints([4000, 10]), mask.cuda(), out)
+    op(q, kc, vc, kd, vd, ints([4000, 10]), mask.cuda(), q)
+    assert torch.equal(q, out)
+
+
+def test_results_over_inputs_are_refused():
+    g, n, nkv, hd = gen(61), 6, 2, 64
+    buf = randn(g, n, 4 + nkv + 1, hd)
+    op = PackedAttention(tokens=n, num_seqs=1, num_kv_groups=nkv, q_heads_per_group=2, head_dim=hd)
+    q, v = randn(g, n, 4, hd), randn(g, n, nkv, hd)
+    with pytest.raises(RuntimeError, match="argument"):
+        op(q, buf[:, :nkv], v, ints([0, n]), buf[:, 1:5])
+    op(q, buf[:, :nkv], v, ints([0, n]), buf[:, nkv:nkv + 4])
+    cache, draft = randn(g, 2, 1, nkv, 64, hd), randn(g, 1, 1, 3, nkv, hd)
+    commit = DraftTreeCommit(layers=1, batch=1, nodes=3, max_ctx=64, num_kv_groups=nkv, head_dim=hd)
+    tree, row = [ints([[0, 0, 0]]) for _ in range(4)], [ints([0]) for _ in range(4)]
+    inside = cache[0:1, :, :, 10:13].transpose(2, 3)
+    for kd, kc in ((inside, cache[0:1]), (draft, cache[1:2])):
+        with pytest.raises(RuntimeError, match="argument"):
+            commit(*tree[:3], row[0], kd, draft, kc, cache[1:2], tree[3], *row[1:])
+    commit(*tree[:3], row[0], draft, draft, cache[0:1], cache[1:2], tree[3], *row[1:])

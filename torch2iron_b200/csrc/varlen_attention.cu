@@ -67,6 +67,7 @@
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 #include "t2b_common.cuh"
 #include "launch.cuh"
@@ -1206,6 +1207,52 @@ extern "C" size_t t2b_varlen_attention_workspace_bytes(int head_dim) {
   return head_dim == 64 || head_dim == 128 ? va_ws_bytes(head_dim) : 0;
 }
 
+// Memory of a tensor: `inner` bytes at every combination of the axes (the
+// greatest stride first, axes of one left out).
+struct VaBox {
+  uintptr_t at;
+  long long inner;
+  int n;
+  long long dim[3], stride[3];
+  VaBox(const void* p, long long bytes, std::initializer_list<std::pair<size_t, size_t>> axes = {})   // (extent, 16-bit stride)
+      : at(reinterpret_cast<uintptr_t>(p)), inner(bytes), n(0) {
+    for (const auto& x : axes) {
+      if (x.first == 1) continue;
+      int i = n++;
+      for (; i > 0 && stride[i - 1] < (long long)x.second * 2; --i) dim[i] = dim[i - 1], stride[i] = stride[i - 1];
+      dim[i] = (long long)x.first, stride[i] = (long long)x.second * 2;
+    }
+  }
+  long long span(int level) const {
+    long long s = inner;
+    for (int i = level; i < n; ++i) s += (dim[i] - 1) * stride[i];
+    return s;
+  }
+};
+// No byte in common: the spans are apart, or both repeat with one stride (rows
+// or heads of one wider tensor) and what they hold of a period is apart.
+// `d`: from a's start to b's.
+static bool va_apart(const VaBox& a, const VaBox& b, int i, int j, long long d) {
+  if (d >= a.span(i) || d + b.span(j) <= 0) return true;
+  if (i == a.n || j == b.n || a.stride[i] != b.stride[j]) return false;
+  const long long s = a.stride[i], r = ((d % s) + s) % s;
+  if (a.span(i + 1) > s || b.span(j + 1) > s) return false;
+  return va_apart(a, b, i + 1, j + 1, r) && va_apart(a, b, i + 1, j + 1, r - s);
+}
+static bool va_apart(const VaBox& a, const VaBox& b) { return va_apart(a, b, 0, 0, (long long)(b.at - a.at)); }
+// The results overlap neither the inputs nor one another; out may lie on q, row by row.
+static bool va_results_apart(const VaBox& out, const float* lse, size_t lse_values, const VaBox& q, bool same_layout,
+                             std::initializer_list<VaBox> inputs) {
+  if (!(out.at == q.at && same_layout) && !va_apart(out, q)) return false;
+  for (const VaBox& x : inputs)
+    if (!va_apart(out, x)) return false;
+  if (!lse) return true;
+  const VaBox sums(lse, (long long)lse_values * 4);
+  for (const VaBox& x : inputs)
+    if (!va_apart(sums, x)) return false;
+  return va_apart(sums, out) && va_apart(sums, q);
+}
+
 static int va_check(const void* q, const void* k, const void* v, const void* out, int dtype, int out_dtype, int rows,
                     int n_heads, int n_kv, int head_dim, float scale, std::initializer_list<size_t> strides) {
   if (!q || !k || !v || !out) return T2B_ERR_ARG;
@@ -1233,6 +1280,14 @@ extern "C" int t2b_packed_attention(const void* q, const void* k, const void* v,
   if (!q_start) return T2B_ERR_ARG;
   if (n_seqs < 1 || n_seqs > VA_MAX_KEYS || kv_tokens < 1 || kv_tokens > VA_MAX_KEYS || kv_seqs < 0) return T2B_ERR_SHAPE;
   if (kv_seqs ? (kv_seqs < n_seqs || !k_len || k_start) : (k_start == nullptr) != (k_len == nullptr)) return T2B_ERR_ARG;
+  const size_t heads = n_heads, kv_heads = n_kv, rows = total_q, keys = kv_tokens, bytes = 2 * (size_t)head_dim;
+  const size_t cache_rows = kv_seqs ? kv_seqs : 1;
+  if (!va_results_apart(VaBox(out, bytes, {{rows, o_row}, {heads, o_head}}), lse, rows * heads,
+                        VaBox(q, bytes, {{rows, q_row}, {heads, q_head}}),
+                        (rows == 1 || q_row == o_row) && (heads == 1 || q_head == o_head),
+                        {VaBox(k, bytes, {{cache_rows, k_seq}, {keys, k_tok}, {kv_heads, k_head}}),
+                         VaBox(v, bytes, {{cache_rows, v_seq}, {keys, v_tok}, {kv_heads, v_head}})}))
+    return T2B_ERR_ARG;
   VaParams P{};
   const bool f16 = dtype == T2B_DTYPE_F16;
   P.out = out, P.lse = lse, P.out_f16 = out_dtype == T2B_DTYPE_F16;
@@ -1246,9 +1301,8 @@ extern "C" int t2b_packed_attention(const void* q, const void* k, const void* v,
   if (!k_len) units = std::min(units, va_most_units_own(total_q, live, P.tpt, n_kv));
   const int sized = va_check_sizes(head_dim, units, workspace, workspace_bytes);
   if (sized != T2B_OK) return sized;
-  const size_t seqs = kv_seqs ? kv_seqs : 1;
-  if (!va_kv_map(&P.kmap, f16, k, head_dim, kv_tokens, n_kv, seqs, k_tok, k_head, k_seq) ||
-      !va_kv_map(&P.vmap, f16, v, head_dim, kv_tokens, n_kv, seqs, v_tok, v_head, v_seq))
+  if (!va_kv_map(&P.kmap, f16, k, head_dim, kv_tokens, n_kv, cache_rows, k_tok, k_head, k_seq) ||
+      !va_kv_map(&P.vmap, f16, v, head_dim, kv_tokens, n_kv, cache_rows, v_tok, v_head, v_seq))
     return T2B_ERR_ARG;
   P.q_start = q_start, P.k_start = k_start, P.k_len = k_len;
   P.scale_log2 = scale * 1.4426950408889634f;
@@ -1269,6 +1323,15 @@ extern "C" int t2b_tree_attention(const void* q, const void* k_cache, const void
   if (rc != T2B_OK) return rc;
   if (!k_draft || !v_draft || !ctx_len || !mask) return T2B_ERR_ARG;
   if (va_misaligned(k_draft) || va_misaligned(v_draft) || (reinterpret_cast<uintptr_t>(mask) & 7)) return T2B_ERR_ALIGN;
+  const size_t rows = (size_t)B * T, nodes = T, heads = n_heads, kv_heads = n_kv, batch = B, bytes = 2 * (size_t)head_dim;
+  const long long cache = (long long)batch * kv_heads * max_ctx * bytes;
+  if (!va_results_apart(VaBox(out, bytes, {{rows, o_row}, {heads, o_head}}), lse, rows * heads,
+                        VaBox(q, bytes, {{rows, q_row}, {heads, q_head}}),
+                        (rows == 1 || q_row == o_row) && (heads == 1 || q_head == o_head),
+                        {VaBox(k_cache, cache), VaBox(v_cache, cache),
+                         VaBox(k_draft, bytes, {{batch, kd_row}, {nodes, kd_node}, {kv_heads, kd_head}}),
+                         VaBox(v_draft, bytes, {{batch, vd_row}, {nodes, vd_node}, {kv_heads, vd_head}})}))
+    return T2B_ERR_ARG;
   VaParams P{};
   const bool f16 = dtype == T2B_DTYPE_F16;
   P.out = out, P.lse = lse, P.out_f16 = out_dtype == T2B_DTYPE_F16;

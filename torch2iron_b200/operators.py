@@ -491,7 +491,8 @@ class PackedAttention:
     are cache rows ``[num_seqs, num_kv_groups, max_ctx, head_dim]`` and ``k_len``
     says how many of each row count, the sequence's own queries among them.
     A query without keys gets zeros (and ``lse`` -inf); rows of ``out`` and
-    ``lse`` outside every sequence keep what they held.  A call that could have
+    ``lse`` outside every sequence keep what they held.  ``out`` may be ``q``
+    itself, and otherwise shares no memory with the inputs.  A call that could have
     more than 2^31 - 1 units of work (``t2b_packed_attention``; one prompt of 1.4
     million tokens at 32 over 8 heads) is refused."""
 
@@ -618,7 +619,8 @@ class DraftTreeAttention:
     drafted nodes whose bit is set in ``mask[b, i]`` (``draft_tree``); the
     drafted K/V stay outside the cache until ``DraftTreeCommit`` moves the
     accepted ones.  Nodes from ``num_nodes[b]`` on are not computed: their rows
-    of ``out`` and ``lse`` keep what they held."""
+    of ``out`` and ``lse`` keep what they held.  ``out`` may be ``q`` itself, and
+    otherwise shares no memory with the inputs."""
 
     batch: int
     nodes: int
@@ -707,9 +709,9 @@ class DraftTreeCommit:
     are ``[layers, batch, nodes, kv, head_dim]`` or a sequence of one tensor per
     layer, ``k_caches`` / ``v_caches`` likewise ``[layers, batch, kv, max_ctx,
     head_dim]``.  Writes ``path`` (-1 behind the walk's end), ``num_accepted``,
-    ``next_token`` and ``new_len = ctx_len + num_accepted``, none of them one of
-    the inputs; a row with no live node or no room accepts nothing (next token
-    -1)."""
+    ``next_token`` and ``new_len = ctx_len + num_accepted``; they and the caches
+    share no memory with the drafts, the other inputs or one another.  A row with
+    no live node or no room accepts nothing (next token -1)."""
 
     layers: int
     batch: int
