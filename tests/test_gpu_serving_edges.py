@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests.serving_ref import assert_attention, attention_rows
-from tests.test_gpu_serving import gen, ints, randn
+from tests.test_gpu_serving import check_packed, gen, ints, randn
 from torch2iron_b200.operators import DraftTreeAttention, DraftTreeCommit, PackedAttention, draft_tree
 
 pytestmark = pytest.mark.gpu
@@ -176,3 +176,92 @@ def test_results_over_inputs_are_refused():
         with pytest.raises(RuntimeError, match="argument"):
             commit(*tree[:3], row[0], kd, draft, kc, cache[1:2], tree[3], *row[1:])
     commit(*tree[:3], row[0], draft, draft, cache[0:1], cache[1:2], tree[3], *row[1:])
+
+
+@pytest.mark.parametrize("S,long", [(640, ()), (641, (0, 640)), (1500, (639, 640, 1281)), (1500, (1499,))])
+def test_packed_more_sequences_than_threads(S, long):
+    """The list's start is counted 640 sequences at a time: empty ones beside that
+    border, and some long enough to be cut between CTAs."""
+    n = [(i * 7) % 4 for i in range(S)]
+    for i in (638, 639, 640, 641, 1279, 1280):
+        if i < S:
+            n[i] = 0
+    for i in long:
+        n[i] = 3000
+    check_packed(n, (2, 1, 64), extra_rows=5)
+
+
+def test_packed_one_prompt_of_more_pairs_than_half_the_threads():
+    """128 query heads on one key head make a pair of two tokens: each thread looks for a cut in several pairs."""
+    check_packed([3, 1500, 0, 700], (128, 1, 64), extra_rows=1)
+
+
+def test_packed_one_prompt_of_more_than_20480_tokens():
+    """The same with 4 query heads per key head (64 tokens a pair); the reference of some rows."""
+    n, nh, nkv, hd = 22001, 4, 1, 64
+    g = gen(70)
+    q, k, v = randn(g, n, nh, hd, scale=1.5), randn(g, n, nkv, hd), randn(g, n, nkv, hd)
+    out, lse = torch.full_like(q, math.nan), torch.full((n, nh), math.nan, device="cuda")
+    op = PackedAttention(tokens=n, num_seqs=1, num_kv_groups=nkv, q_heads_per_group=nh, head_dim=hd)
+    op(q, k, v, ints([0, n]), out, lse=lse)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    rows = torch.tensor([0, 63, 64, 127, 128, 5000, 10239, 10240, 20479, 20480, 20543, 20544, 21951, 21952, 22000])
+    seen = torch.arange(n)[None] <= rows[:, None]
+    assert_attention(out[rows], lse[rows], attention_rows(q[rows], k, v, seen, op.scale))
+
+
+def test_calls_without_any_row_write_nothing():
+    g, nkv, hd = gen(71), 2, 64
+    q, kv = randn(g, 9, 4, hd), randn(g, 9, nkv, hd)
+    for S in (1, 5, 700):
+        op = PackedAttention(tokens=9, num_seqs=S, num_kv_groups=nkv, q_heads_per_group=2, head_dim=hd)
+        for start in (0, 4, 9):
+            out, lse = torch.full_like(q, 7.0), torch.full((9, 4), 7.0, device="cuda")
+            op(q, kv, kv, ints([start] * (S + 1)), out, lse=lse)
+            assert (out == 7).all() and (lse == 7).all()
+    B, T = 3, 5
+    q, kd, cache = randn(g, B, T, 4, hd), randn(g, B, T, nkv, hd), randn(g, B, nkv, 64, hd)
+    out, lse = torch.full_like(q, 7.0), torch.full((B, T, 4), 7.0, device="cuda")
+    mask = torch.ones(B, T, 1, dtype=torch.int64, device="cuda")
+    op = DraftTreeAttention(batch=B, nodes=T, max_ctx=64, num_kv_groups=nkv, q_heads_per_group=2, head_dim=hd)
+    for live in ([0, 0, 0], [-3, 0, -1]):
+        op(q, cache, cache, kd, kd, ints([64, 0, 9]), mask, out, num_nodes=ints(live), lse=lse)
+        assert (out == 7).all() and (lse == 7).all()
+
+
+def test_packed_starts_outside_the_tensors_are_clamped_to_their_rows():
+    """The rows that the clamped starts leave have their values, the others are not written."""
+    g, nkv, hd = gen(72), 2, 64
+    q, k, v = randn(g, 10, 4, hd), randn(g, 40, nkv, hd), randn(g, 40, nkv, hd)
+    op = PackedAttention(tokens=10, num_seqs=3, num_kv_groups=nkv, q_heads_per_group=2, head_dim=hd, kv_tokens=40)
+    out, lse = torch.full_like(q, math.nan), torch.full((10, 4), math.nan, device="cuda")
+    op(q, k, v, ints([-5, 2, 2, 2000000000]), out, k_start=ints([0, 3, 5]), k_len=ints([7, 1, 9]), lse=lse)
+    for rows, n, first, k_len in ((slice(0, 2), 2, 0, 7), (slice(2, 10), 8, 5, 9)):
+        seen = torch.arange(k_len)[None] <= k_len - n + torch.arange(n)[:, None]
+        keys = slice(first, first + k_len)
+        assert_attention(out[rows], lse[rows], attention_rows(q[rows], k[keys], v[keys], seen, op.scale))
+    out.fill_(7.0)
+    op(q, k, v, ints([4, 4, 6, 6]), out, k_start=ints([0, 30, 0]), k_len=ints([7, 2000000000, 9]), lse=lse)
+    assert (out[:4] == 7).all() and (out[6:] == 7).all()
+    assert_attention(out[4:6], None, attention_rows(q[4:6], k[30:], v[30:], torch.ones(2, 10, dtype=torch.bool), op.scale))
+
+
+def test_commit_of_fp16_caches():
+    g, L, B, T, nkv, hd, ctx = gen(73), 3, 2, 6, 2, 128, 64
+    kd, vd = randn(g, L, B, T, nkv, hd, dtype=HF), randn(g, L, B, T, nkv, hd, dtype=HF)
+    kc, vc = randn(g, L, B, nkv, ctx, hd, dtype=HF), randn(g, L, B, nkv, ctx, hd, dtype=HF)
+    want = [kc.clone(), vc.clone()]
+    parents, tokens, predicted = [[-1, 0, 1, 1, 3, 4]] * 2, [[9, 1, 2, 3, 4, 5]] * 2, [[1, 3, 0, 4, 5, 8], [7] * 6]
+    out = [ints([[0] * T] * B)] + [ints([0] * B) for _ in range(3)]
+    DraftTreeCommit(layers=L, batch=B, nodes=T, max_ctx=ctx, num_kv_groups=nkv, head_dim=hd, dtype=HF)(
+        ints(tokens), ints(parents), ints(predicted), ints([20, 63]), kd, vd, kc, vc, *out)
+    paths = [[0, 1, 3, 4, 5], [0]]
+    for b, at in ((0, 20), (1, 63)):
+        for i, n in enumerate(paths[b]):
+            want[0][:, b, :, at + i], want[1][:, b, :, at + i] = kd[:, b, n], vd[:, b, n]
+        assert out[0][b].tolist() == paths[b] + [-1] * (T - len(paths[b]))
+    assert out[2].tolist() == [8, 7] and out[3].tolist() == [25, 64]
+    assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+    with pytest.raises(ValueError):
+        DraftTreeCommit(layers=L, batch=B, nodes=T, max_ctx=ctx, num_kv_groups=nkv, head_dim=hd)(
+            ints(tokens), ints(parents), ints(predicted), ints([20, 63]), kd, vd, kc, vc, *out)
