@@ -1,10 +1,12 @@
 """Host checks of the serving operators beyond their first tests."""
 
 import ctypes as C
+import math
 
 import pytest
 
 from torch2iron_b200 import _lib
+from torch2iron_b200.operators import draft_tree
 
 ERR_SHAPE, ERR_ALIGN, ERR_ARG, ERR_WORKSPACE = 1, 2, 6, 5
 
@@ -120,3 +122,10 @@ def test_tree_commit_refuses_caches_over_drafts_and_over_one_another(base):
                 dict(kc=[kc[0], kc[0], kc[2]]), dict(vc=kc), dict(kc=[kc[2], kc[1], kc[0] + cache // 2]), dict(vc=[*vc[:2], vd[1]]),
                 dict(path=kc[1] + 32), dict(path=vd[2] + 32)):
         assert call(**bad) == ERR_ARG, bad
+
+
+@pytest.mark.parametrize("live", [[1.5, 2.0], [math.nan, 2.0], ["1", "2"]])
+def test_draft_tree_takes_whole_numbers_of_nodes(live):
+    with pytest.raises(ValueError):
+        draft_tree([[-1, 0], [-1, 0]], live)
+    assert draft_tree([[-1, 0], [-1, 0]], [1.0, 2.0])[0].tolist() == [[[1], [0]], [[1], [3]]]

@@ -587,8 +587,8 @@ def draft_tree(parents, num_nodes=None) -> tuple[torch.Tensor, torch.Tensor]:
     B, T = par.shape
     live = np.full(B, T) if num_nodes is None else \
         np.asarray(num_nodes.cpu() if isinstance(num_nodes, torch.Tensor) else num_nodes).reshape(-1)
-    if live.shape != (B,) or live.min(initial=0) < 0 or live.max(initial=0) > T:
-        raise ValueError(f"num_nodes must be {B} values in 0..{T}")
+    if live.shape != (B,) or live.dtype.kind not in "biuf" or not ((live >= 0) & (live <= T) & (live == np.trunc(live))).all():
+        raise ValueError(f"num_nodes must be {B} whole numbers in 0..{T}")
     node = np.arange(T)
     used = node[None] < live[:, None]
     if (used & (node[None] > 0) & ((par < 0) | (par >= node[None]))).any():
