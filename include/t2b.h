@@ -421,14 +421,15 @@ T2B_API int t2b_argmax_rows(const void* logits, int dtype, int M, int V, int ld,
  * argument, out_dtype (bf16 or fp16) that of out; strides are in elements,
  * nonzero multiples of 8; bases are 16-byte aligned; the innermost (head_dim)
  * axis is contiguous; head_dim 64 or 128; up to 128 q heads per kv head;
- * scale > 0 multiplies q . k.  lse (may be NULL) is fp32 [rows][n_heads], the
- * natural log of the softmax sum.  A row that sees no key gets out = 0 and
- * lse = -inf.  Values of K and V that no row of the call sees may be anything,
- * infinities and NaN among them; so may a K value in the rows that do not see
- * its key.  An infinity or NaN in a V value that some row sees may reach the
- * other rows of its sequence too (0 times it is not 0).  The lengths, starts and masks are read on
- * the device; what lies outside the given extents is ignored (clamped), and
- * output rows that belong to no sequence or to no live node are not written.
+ * scale > 0 multiplies q . k (scale * log2(e) is finite in 32 bits).  lse (may
+ * be NULL) is fp32 [rows][n_heads], the natural log of the softmax sum.  A row
+ * that sees no key gets out = 0 and lse = -inf.  Values of K and V that no row
+ * of the call sees may be anything, infinities and NaN among them; so may a K
+ * value in the rows that do not see its key.  An infinity or NaN in a V value
+ * that some row sees may reach the other rows of its sequence too (0 times it is
+ * not 0).  The lengths, starts and masks are read on the device; what lies
+ * outside the given extents is ignored (clamped), and output rows that belong to
+ * no sequence or to no live node are not written.
  * out and lse share no memory with q, K, V or one another (T2B_ERR_ARG), except
  * that out may be q itself, with q's strides; views that interleave (heads of
  * one wider tensor) are told apart where they have their strides in common.

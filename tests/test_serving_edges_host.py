@@ -6,7 +6,7 @@ import math
 import pytest
 
 from torch2iron_b200 import _lib
-from torch2iron_b200.operators import draft_tree
+from torch2iron_b200.operators import DraftTreeAttention, PackedAttention, draft_tree
 
 ERR_SHAPE, ERR_ALIGN, ERR_ARG, ERR_WORKSPACE = 1, 2, 6, 5
 
@@ -129,3 +129,16 @@ def test_draft_tree_takes_whole_numbers_of_nodes(live):
     with pytest.raises(ValueError):
         draft_tree([[-1, 0], [-1, 0]], live)
     assert draft_tree([[-1, 0], [-1, 0]], [1.0, 2.0])[0].tolist() == [[[1], [0]], [[1], [3]]]
+
+
+@pytest.mark.parametrize("scale", [3e38, 1e39, 1e-60])
+def test_a_scale_has_to_fit_the_kernels_fp32(base, scale):
+    """The kernels multiply by scale * log2(e) in 32 bits."""
+    with pytest.raises(ValueError):
+        PackedAttention(tokens=4, num_seqs=1, scale=scale)
+    with pytest.raises(ValueError):
+        DraftTreeAttention(batch=1, nodes=4, max_ctx=64, scale=scale)
+    far = [base + (i << 20) for i in range(5)]
+    got = _lib.load().t2b_packed_attention(*far[:4], None, 0, 0, far[4], None, None, 1, 4, 0, 4, 4, 2, 64, 256, 64, 256, 64, 128,
+                                           64, 8, 128, 64, 8, scale, None, 0, None)
+    assert got == ERR_ARG

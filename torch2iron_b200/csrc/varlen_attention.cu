@@ -1258,7 +1258,7 @@ static int va_check(const void* q, const void* k, const void* v, const void* out
   if (!q || !k || !v || !out) return T2B_ERR_ARG;
   if ((dtype != T2B_DTYPE_BF16 && dtype != T2B_DTYPE_F16) || (out_dtype != T2B_DTYPE_BF16 && out_dtype != T2B_DTYPE_F16))
     return T2B_ERR_ARG;
-  if (!(scale > 0.f) || !isfinite(scale)) return T2B_ERR_ARG;
+  if (!(scale > 0.f) || !isfinite(scale * 1.4426950408889634f)) return T2B_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return T2B_ERR_SHAPE;
   if (rows < 1 || rows > VA_MAX_KEYS || n_kv < 1 || n_heads < 1 || n_heads % n_kv || n_heads / n_kv > 128) return T2B_ERR_SHAPE;
   if (va_misaligned(q) || va_misaligned(k) || va_misaligned(v) || va_misaligned(out)) return T2B_ERR_ALIGN;

@@ -475,8 +475,8 @@ def _check_heads(op) -> None:
         raise ValueError("out_dtype must be torch.bfloat16 or torch.float16")
     if op.scale is None:
         op.scale = 1.0 / math.sqrt(op.head_dim)
-    if not (op.scale > 0 and math.isfinite(op.scale)):
-        raise ValueError("scale must be positive and finite")
+    if not 2.0 ** -149 <= op.scale < 2.0 ** 127:      # the kernels' fp32 scale * log2(e)
+        raise ValueError("scale must be positive and finite in 32 bits")
 
 
 @dataclass
