@@ -435,7 +435,9 @@ T2B_API int t2b_argmax_rows(const void* logits, int dtype, int M, int V, int ld,
  * one wider tensor) are told apart where they have their strides in common.
  * The workspace (t2b_varlen_attention_workspace_bytes) needs no
  * initialisation and is 256-byte aligned; calls that share one must be
- * ordered on one stream.
+ * ordered on one stream.  The status returned is the launch's: a device wait that
+ * ran out leaves rows of the attention unwritten or half written, and only the
+ * stream's or thread's status word says so (t2b_bind_error_word).
  */
 T2B_API size_t t2b_varlen_attention_workspace_bytes(int head_dim);
 

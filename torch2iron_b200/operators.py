@@ -494,7 +494,9 @@ class PackedAttention:
     ``lse`` outside every sequence keep what they held.  ``out`` may be ``q``
     itself, and otherwise shares no memory with the inputs.  A call that could have
     more than 2^31 - 1 units of work (``t2b_packed_attention``; one prompt of 1.4
-    million tokens at 32 over 8 heads) is refused."""
+    million tokens at 32 over 8 heads) is refused.  A device wait that ran out is
+    seen in the status word bound to the stream (``_lib.status_word``), and there
+    alone; its rows are not to be used."""
 
     tokens: int
     num_seqs: int
@@ -620,7 +622,8 @@ class DraftTreeAttention:
     drafted K/V stay outside the cache until ``DraftTreeCommit`` moves the
     accepted ones.  Nodes from ``num_nodes[b]`` on are not computed: their rows
     of ``out`` and ``lse`` keep what they held.  ``out`` may be ``q`` itself, and
-    otherwise shares no memory with the inputs."""
+    otherwise shares no memory with the inputs.  A device wait that ran out is
+    seen in the stream's status word, as for ``PackedAttention``."""
 
     batch: int
     nodes: int
