@@ -13,10 +13,11 @@
 // so there is no workspace and the result is the same every time.  A thread
 // holds 32 values of a chunk in registers, so the maximum is known before the
 // exponentials and the running sums are rescaled once per chunk.  All sums are
-// fp32.  Measured: 1500 rows of 151936 fp32 183 us = 5.0 TB/s (0.76 of the
-// measured copy; three CTAs per SM wait for their loads); one row with 20
-// alternatives 13 us, of which the alternatives' barriers and rankings are
-// about half.
+// fp32.  Measured: 1500 rows of 151936 fp32 188 us a call = 4.85 TB/s (0.74 of
+// the measured copy; three CTAs per SM wait for their loads, at 80 registers
+// with 28 to 32 bytes of spill stores a thread, and the rows are 3.4 waves of
+// CTAs); one row with 20 alternatives 12 us a call, of which the alternatives'
+// barriers and rankings are about half.
 //
 // Alternatives: a value and its index form one 64-bit key (order-preserving
 // value bits << 32 | ~index: larger value first, ties to the lower index).

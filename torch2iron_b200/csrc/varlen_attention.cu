@@ -17,8 +17,10 @@
 // lengths, long contexts with few rows and single tokens balance alike without
 // the host knowing a length.  An item cut between CTAs leaves fp32 partials
 // (output, maximum, sum) that a second kernel joins in a fixed order; items of
-// up to VA_SNAP blocks are not cut.  (24 ragged prompts: 276 us with blocks
-// alone counted, 174 us with the items' own cost.)
+// up to VA_SNAP blocks are not cut.  (24 ragged prompts, replays of a graph: 276
+// us with blocks alone counted, 180 us with the items' own cost.)  The cut, and
+// with it the order of a row's sums, follows from the whole call: the same call
+// repeats its bits, the same row in another call need not.
 //
 // CTA: two softmax groups of eight warps, a TMA warp and an MMA warp.
 //   S_t = Q_t K^T     A, B from shared memory (128-byte swizzled TMA tiles)
@@ -34,16 +36,20 @@
 //
 // Bound.  A block of two tiles of head_dim 128 is 2048 clocks of MMAs and 2048
 // of exponentials (16 a clock) for 64 KB of K and V, which HBM brings in 2700:
-// long prompts are bound by the products, few rows over a long context by
-// HBM.  Measured (head_dim 128, 32 over 8 heads): prompts of 3600, 6830 and
-// 12001 tokens 1.42 ms = 1.18 PFLOP/s, the MMA pipe busy 62 % and the
-// special-function unit 62 % of the cycles; a block takes 3100 clocks, since a
-// tile's two products and its softmax wait for one another and two tiles do
-// not hide that wholly.  Trees of 63 nodes over 60001 and 45001 keys 118 us =
-// 3.7 TB/s.  Tried and not kept: one softmax warpgroup per tile (1600 against
-// 1414 us on the prompts), part of the exponentials as polynomials on the FMA
-// pipes (no gain: packed FMAs take two slots), scores kept in registers
-// instead of read twice (spills; 1.60 against 1.44 ms).
+// the floor is the products for long prompts and HBM for few rows over a long
+// context.  No unit is full: a block takes 3100 clocks, since a tile's two
+// products and its softmax wait for one another and two tiles do not hide that
+// wholly.  Measured (head_dim 128, 32 over 8 heads): prompts of 3600, 6830 and
+// 12001 tokens 1.65 ms a call in a loop = 1.01 PFLOP/s (one launch on a cool
+// GPU 1.38 ms = 1.21), the MMA pipe and the special-function unit each busy 62 %
+// of the cycles; trees of 63 nodes over 60001 and 45001 keys 142 us a call = 3.05
+// TB/s, both at 54 %; trees of 21 nodes at head_dim 64 64 us = 3.3 TB/s, the
+// special-function unit at 50 % and the MMA pipe at 25 %.  Tried and not kept:
+// one softmax warpgroup per tile (1600 against 1414 us on the prompts), part of
+// the exponentials as polynomials on the FMA pipes (no gain: packed FMAs take
+// two slots), scores kept in registers instead of read twice (1.60 against 1.44
+// ms, more spills; ptxas reports 72 to 88 bytes of spill stores a thread as it
+// is, at the 96 registers that 640 threads leave).
 //
 // Numerics.  Scores, maxima, sums and O are fp32; the weights are rounded
 // once, to the operands' 16-bit type, as A of the second product (the sum
