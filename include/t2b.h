@@ -432,7 +432,7 @@ T2B_API int t2b_argmax_rows(const void* logits, int dtype, int M, int V, int ld,
  * no sequence or to no live node are not written.
  * out and lse share no memory with q, K, V or one another (T2B_ERR_ARG), except
  * that out may be q itself, with q's strides; views that interleave (heads of
- * one wider tensor) are told apart where they have their strides in common.
+ * one wider tensor) are told apart.
  * The workspace (t2b_varlen_attention_workspace_bytes) needs no
  * initialisation and is 256-byte aligned; calls that share one must be
  * ordered on one stream.  The status returned is the launch's: a device wait that

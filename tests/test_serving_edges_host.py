@@ -89,6 +89,23 @@ def test_packed_attention_takes_views_of_one_fused_tensor(base):
     assert packed(base, base + (1 << 20) + 8 * 128, o_strides=flip, k_strides=flip) == ERR_ARG
 
 
+@pytest.mark.parametrize("rows,nh", [(1, 4), (1, 1), (5, 1), (3, 4)])
+def test_packed_attention_takes_the_last_rows_of_a_fused_tensor_in_place(base, rows, nh):
+    """The last tokens of [q | k | v] rows over all keys there, out in place of q: one row, or one head, has no stride
+    in common with the keys' rows."""
+    base <<= 8
+    nkv, keys, row = 1, 100, (nh + 2) * 64
+
+    def call(out_at):
+        q = base + (keys - rows) * row * 2
+        return _lib.load().t2b_packed_attention(
+            q, base + nh * 128, base + (nh + 1) * 128, q + out_at, None, 0, 0, base + (3 << 20), base + (4 << 20),
+            base + (5 << 20), 1, rows, 0, keys, nh, nkv, 64, row, 64, row, 64, row, 64, 8, row, 64, 8, 0.125, None, 0, None)
+
+    assert call(0) == ERR_WORKSPACE
+    assert call(128) == ERR_ARG and call(-128) == ERR_ARG        # over k, over the v of the row before
+
+
 def tree(base, out, lse=None, kd=None, B=2, T=4, nh=4, nkv=2, hd=64, ctx=64):
     return _lib.load().t2b_tree_attention(
         base, base + (1 << 20), base + (2 << 20), kd or base + (3 << 20), base + (4 << 20), out, lse, 0, 0, base + (5 << 20),

@@ -1235,15 +1235,17 @@ struct VaBox {
     return s;
   }
 };
-// No byte in common: the spans are apart, or both repeat with one stride (rows
-// or heads of one wider tensor) and what they hold of a period is apart.
-// `d`: from a's start to b's.
+// No byte in common: the spans are apart, or what lies in one period of the
+// greater stride is (both repeat with it, as rows or heads of one wider tensor
+// do, or one does and the other lies between).  `d`: from a's start to b's.
 static bool va_apart(const VaBox& a, const VaBox& b, int i, int j, long long d) {
   if (d >= a.span(i) || d + b.span(j) <= 0) return true;
-  if (i == a.n || j == b.n || a.stride[i] != b.stride[j]) return false;
-  const long long s = a.stride[i], r = ((d % s) + s) % s;
-  if (a.span(i + 1) > s || b.span(j + 1) > s) return false;
-  return va_apart(a, b, i + 1, j + 1, r) && va_apart(a, b, i + 1, j + 1, r - s);
+  const long long sa = i < a.n ? a.stride[i] : 0, sb = j < b.n ? b.stride[j] : 0, s = std::max(sa, sb);
+  if (s == 0) return false;
+  i += sa == s, j += sb == s;
+  if (a.span(i) > s || b.span(j) > s) return false;
+  const long long r = ((d % s) + s) % s;
+  return va_apart(a, b, i, j, r) && va_apart(a, b, i, j, r - s);
 }
 static bool va_apart(const VaBox& a, const VaBox& b) { return va_apart(a, b, 0, 0, (long long)(b.at - a.at)); }
 // The results overlap neither the inputs nor one another; out may lie on q, row by row.
